@@ -1,0 +1,187 @@
+// Paged KV cache: storing a ragged batch's rows in their pages (rounded to 16 bits or
+// quantised to Q8) and reading rows back.
+//
+// Both are copies bound by HBM: rows * n_kv_heads * head_dim elements in and out, for K
+// and V.  A row's K (or V) is n_kv_heads * head_dim / 8 pieces of 8 elements, and a wave
+// takes one row (several when a row has fewer than 64 pieces) of K or V, a piece per
+// lane, so both sides move in whole lines.  The wave finds its row's sequence by a
+// 64-ary search of row_start (one load for up to 63 sequences); a row's values are
+// requested before the search so that its latency hides theirs.
+#include "gr_common.hpp"
+#include "paged_internal.hpp"
+
+namespace gr {
+
+constexpr int kPagedKvThreads = 256;
+
+// 8 consecutive elements as floats.
+template <typename T>
+__device__ __forceinline__ void pk_load8(const typename T::storage* src, float* x) {
+    const uint4* p = (const uint4*)src;
+    if constexpr (T::bytes == 4) {
+        const uint4 a = p[0], b = p[1];
+        unpack16<T>(a, x);
+        unpack16<T>(b, x + 4);
+    } else {
+        const uint4 a = p[0];
+        unpack16<T>(a, x);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void pk_store8(typename T::storage* dst, const float* x) {
+    if constexpr (T::bytes == 4) {
+        ((float4*)dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        ((float4*)dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            w[i] = (uint32_t)from_f32<T>(x[2 * i]) | ((uint32_t)from_f32<T>(x[2 * i + 1]) << 16);
+        *(uint4*)dst = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// Where a row of the batch is in the cache: page (or -1: nowhere) and row of it.
+struct PagedPlace {
+    int page, row;
+};
+
+// Row `row` of the lane's, seq: the sequence of a row at or before it in the wave.
+__device__ __forceinline__ PagedPlace pk_place(const PagedSeqs& s, int row, int seq) {
+    PagedPlace at{-1, 0};
+    while (seq < s.n_seq && row >= s.row_start[seq + 1]) seq++;
+    if (seq >= s.n_seq) return {-2, 0};
+    const int end = seq_row(s, seq + 1);
+    const int n = end - seq_row(s, seq);
+    const int pos = seq_len(s, seq, n) - (end - row);
+    if (pos < 0) return at;
+    const int id = s.page_table[(int64_t)seq * s.table_stride + (pos >> s.page_shift)];
+    at.page = (unsigned)id < (unsigned)s.n_pages ? id : -1;
+    at.row = pos & ((1 << s.page_shift) - 1);
+    return at;
+}
+
+// code of x: round(x * inv) with halves away from zero, as quantize_row_q8
+// (inference.rs:249-268); a NaN becomes 0, as Rust's saturating `as i8`.
+__device__ __forceinline__ uint32_t pk_code(float x, float inv) {
+    float r = roundf(x * inv);
+    if (r < -127.0f) r = -127.0f;
+    if (r > 127.0f) r = 127.0f;
+    return (uint32_t)(uint8_t)(int8_t)(int)r;
+}
+
+struct KvQ8 {};
+
+// lanes_per_row lanes (a power of two up to 64) share a row; 64 / lanes_per_row rows a wave.
+template <int D, typename ROWS, typename KV, bool WRITE>
+__global__ __launch_bounds__(kPagedKvThreads) void paged_kv_kernel(const PagedKvLaunch p, const int lanes_per_row) {
+    constexpr int CPH = D / 8;  // pieces per head
+    constexpr bool q8 = std::is_same_v<KV, KvQ8>;
+    const int lane = threadIdx.x & 63;
+    const int unit = (int)blockIdx.x * (kPagedKvThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rpw = 64 / lanes_per_row;
+    const int first = (unit >> 1) * rpw;  // the wave's first row; units alternate between K and V
+    const int which = unit & 1;
+    if (first >= p.seqs.n_rows) return;
+    const int row = first + lane / lanes_per_row;
+    const int n_pieces = p.n_kv_heads * CPH;
+    // the first sequence a row of this wave may belong to (rows in front of every sequence: -1)
+    const int seq0 = seq_of_row(p.seqs, first);
+    PagedPlace at{-2, 0};
+    if (row < p.seqs.n_rows && row >= p.seqs.row_start[0]) at = pk_place(p.seqs, row, max(seq0, 0));
+    if (seq0 < 0 && first >= p.seqs.row_start[0]) return;  // behind the last sequence
+    if (at.page == -2 || (WRITE && at.page < 0)) return;
+    using RT = typename ROWS::storage;
+    RT* const rows = (RT*)p.rows[which] + (int64_t)row * p.rows_row_stride;
+    const int64_t cell = (int64_t)at.page * p.page_stride + (int64_t)at.row * p.row_stride;
+    const int64_t sc0 = (int64_t)at.page * p.scale_page_stride + (int64_t)at.row * p.scale_row_stride;
+    for (int c = lane % lanes_per_row; c < n_pieces; c += lanes_per_row) {
+        const int g = c / CPH, i = (c % CPH) * 8;
+        RT* const r = rows + g * p.rows_head_stride + i;
+        const int64_t e = cell + g * p.head_stride + i;
+        float x[8];
+        if constexpr (WRITE) {
+            pk_load8<ROWS>(r, x);
+            if constexpr (q8) {
+                float amax = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(x[j]));
+                // a head's CPH pieces are CPH adjacent lanes (lanes_per_row is a multiple of CPH)
+#pragma unroll
+                for (int m = CPH / 2; m >= 1; m >>= 1) amax = fmaxf(amax, shfl_xor(amax, m));
+                const float inv = amax == 0.0f ? 0.0f : __fdiv_rn(127.0f, amax);
+                uint32_t w0 = 0, w1 = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    w0 |= pk_code(x[j], inv) << (8 * j);
+                    w1 |= pk_code(x[j + 4], inv) << (8 * j);
+                }
+                *(uint2*)((int8_t*)p.pages[which] + e) = make_uint2(w0, w1);
+                if (i == 0)
+                    p.scale[which][sc0 + g * p.scale_head_stride] = amax == 0.0f ? 1.0f : __fdiv_rn(amax, 127.0f);
+            } else {
+                pk_store8<KV>((typename KV::storage*)p.pages[which] + e, x);
+            }
+        } else {
+            if (at.page < 0) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = 0.0f;
+            } else if constexpr (q8) {
+                const uint2 w = *(const uint2*)((const int8_t*)p.pages[which] + e);
+                const float s = p.scale[which][sc0 + g * p.scale_head_stride];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[j] = (float)(int8_t)(w.x >> (8 * j)) * s;
+                    x[j + 4] = (float)(int8_t)(w.y >> (8 * j)) * s;
+                }
+            } else {
+                pk_load8<KV>((const typename KV::storage*)p.pages[which] + e, x);
+            }
+            pk_store8<ROWS>(r, x);
+        }
+    }
+}
+
+template <int D, typename ROWS, typename KV, bool WRITE>
+static hipError_t launch_kv(const PagedKvLaunch& p, hipStream_t st) {
+    const int pieces = p.n_kv_heads * (D / 8);
+    int lpr = 64;
+    while (lpr > D / 8 && lpr / 2 >= pieces) lpr /= 2;
+    const int64_t units = 2 * (((int64_t)p.seqs.n_rows + 64 / lpr - 1) / (64 / lpr));
+    const int64_t wgs = (units + kPagedKvThreads / 64 - 1) / (kPagedKvThreads / 64);
+    paged_kv_kernel<D, ROWS, KV, WRITE><<<dim3((unsigned)wgs), kPagedKvThreads, 0, st>>>(p, lpr);
+    return hipGetLastError();
+}
+
+template <int D, typename ROWS, bool WRITE>
+static hipError_t launch_kv_d(const PagedKvLaunch& p, hipStream_t st) {
+    switch (p.kv_dtype) {
+        case GR_DTYPE_F16: return launch_kv<D, ROWS, F16, WRITE>(p, st);
+        case GR_DTYPE_BF16: return launch_kv<D, ROWS, BF16, WRITE>(p, st);
+        default: return launch_kv<D, ROWS, KvQ8, WRITE>(p, st);
+    }
+}
+
+template <typename ROWS, bool WRITE>
+static hipError_t launch_kv_rows(const PagedKvLaunch& p, hipStream_t st) {
+    switch (p.head_dim) {
+        case 64: return launch_kv_d<64, ROWS, WRITE>(p, st);
+        case 128: return launch_kv_d<128, ROWS, WRITE>(p, st);
+        default: return launch_kv_d<256, ROWS, WRITE>(p, st);
+    }
+}
+
+template <bool WRITE>
+static hipError_t launch_kv_any(const PagedKvLaunch& p, hipStream_t st) {
+    switch (p.rows_dtype) {
+        case GR_DTYPE_F32: return launch_kv_rows<F32, WRITE>(p, st);
+        case GR_DTYPE_F16: return launch_kv_rows<F16, WRITE>(p, st);
+        default: return launch_kv_rows<BF16, WRITE>(p, st);
+    }
+}
+
+hipError_t launch_paged_kv_write(const PagedKvLaunch& p, hipStream_t st) { return launch_kv_any<true>(p, st); }
+hipError_t launch_paged_kv_read(const PagedKvLaunch& p, hipStream_t st) { return launch_kv_any<false>(p, st); }
+
+}  // namespace gr

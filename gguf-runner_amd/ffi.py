@@ -1,6 +1,6 @@
-"""ctypes bindings of libgr_attn.so (include/gr_attn.h).
+"""ctypes bindings of libgr_attn.so (include/gr_attn.h, include/gr_paged.h).
 
-The structs below mirror the header field for field.  Nothing here computes
+The structs below mirror the headers field for field.  Nothing here computes
 attention: every call goes to the HIP kernels, and loading fails loudly when the
 library has not been built.
 """
@@ -13,6 +13,7 @@ import pathlib
 PKG_DIR = pathlib.Path(__file__).resolve().parent
 LIB_PATH = pathlib.Path(os.environ.get("GR_ATTN_LIB") or PKG_DIR / "_build" / "libgr_attn.so")
 HEADER = PKG_DIR.parent / "include" / "gr_attn.h"
+PAGED_HEADER = PKG_DIR.parent / "include" / "gr_paged.h"
 
 GR_OK = 0
 GR_ERR_ARG = -1
@@ -72,6 +73,44 @@ class DeltaNetArgs(ctypes.Structure):
     ]
 
 
+class PagedCacheDesc(ctypes.Structure):
+    _fields_ = [
+        ("n_pages", _i32), ("page_size", _i32), ("n_kv_heads", _i32), ("head_dim", _i32),
+        ("kv_dtype", _i32), ("k_pages", _p), ("v_pages", _p), ("page_stride", _i64),
+        ("row_stride", _i64), ("head_stride", _i64), ("k_scale", _p), ("v_scale", _p),
+        ("scale_page_stride", _i64), ("scale_row_stride", _i64), ("scale_head_stride", _i64),
+    ]
+
+
+class PagedBatchDesc(ctypes.Structure):
+    _fields_ = [
+        ("n_seq", _i32), ("n_rows", _i32), ("max_rows", _i32), ("max_len", _i32), ("row_start", _p),
+        ("kv_len", _p), ("page_table", _p), ("table_stride", _i64), ("table_pages", _i32),
+    ]
+
+
+class PagedRows(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("k", _p), ("v", _p), ("row_stride", _i64), ("head_stride", _i64)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("n_heads", _i32), ("dtype", _i32), ("window", _i32), ("score_scale", _f), ("q", _p),
+        ("q_row_stride", _i64), ("q_head_stride", _i64), ("out", _p), ("out_row_stride", _i64),
+        ("out_head_stride", _i64), ("workspace", _p),
+    ]
+
+
+class PackedArgs(ctypes.Structure):
+    _fields_ = [
+        ("n_seq", _i32), ("n_rows", _i32), ("max_rows", _i32), ("n_heads", _i32), ("n_kv_heads", _i32),
+        ("head_dim", _i32), ("dtype", _i32), ("window", _i32), ("score_scale", _f), ("seq_start", _p),
+        ("q", _p), ("q_row_stride", _i64), ("q_head_stride", _i64), ("k", _p), ("v", _p),
+        ("kv_row_stride", _i64), ("kv_head_stride", _i64), ("out", _p), ("out_row_stride", _i64),
+        ("out_head_stride", _i64), ("workspace", _p),
+    ]
+
+
 DELTANET_AUTO, DELTANET_RECURRENT, DELTANET_CHUNKED = 0, 1, 2
 
 
@@ -126,6 +165,19 @@ def _declare(L: ctypes.CDLL) -> None:
     L.gr_deltanet_workspace_size.restype = ctypes.c_size_t
     L.gr_deltanet_attention.argtypes = [ctypes.POINTER(DeltaNetArgs), _p]
     L.gr_deltanet_attention.restype = ctypes.c_int
+    cache, batch, rows = (ctypes.POINTER(t) for t in (PagedCacheDesc, PagedBatchDesc, PagedRows))
+    L.gr_paged_kv_write.argtypes = [cache, batch, rows, _p]
+    L.gr_paged_kv_write.restype = ctypes.c_int
+    L.gr_paged_kv_read.argtypes = [cache, batch, rows, _p]
+    L.gr_paged_kv_read.restype = ctypes.c_int
+    L.gr_paged_attention_workspace_size.argtypes = [cache, batch, ctypes.POINTER(PagedAttentionArgs)]
+    L.gr_paged_attention_workspace_size.restype = ctypes.c_size_t
+    L.gr_paged_attention.argtypes = [cache, batch, ctypes.POINTER(PagedAttentionArgs), _p]
+    L.gr_paged_attention.restype = ctypes.c_int
+    L.gr_packed_attention_workspace_size.argtypes = [ctypes.POINTER(PackedArgs)]
+    L.gr_packed_attention_workspace_size.restype = ctypes.c_size_t
+    L.gr_packed_attention.argtypes = [ctypes.POINTER(PackedArgs), _p]
+    L.gr_packed_attention.restype = ctypes.c_int
     ip = ctypes.c_int
     L.gr_malloc_run_state.argtypes = [ctypes.POINTER(AttnConfig), ctypes.POINTER(_p)]
     L.gr_malloc_run_state.restype = ip
@@ -168,8 +220,8 @@ def check(rc: int) -> None:
 
 
 def header_symbols() -> list[str]:
-    """Function names declared in include/gr_attn.h."""
+    """Function names declared in include/gr_attn.h and include/gr_paged.h."""
     import re
-    text = HEADER.read_text()
+    text = HEADER.read_text() + PAGED_HEADER.read_text()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     return sorted(set(re.findall(r"\b(gr_[a-z0-9_]+)\s*\(", text)))

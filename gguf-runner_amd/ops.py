@@ -267,3 +267,223 @@ class DeltaNetCall:
 
     def __call__(self, stream=None) -> None:
         ffi.check(ffi.lib().gr_deltanet_attention(ctypes.byref(self.args), _stream(stream)))
+
+
+# ---------------------------------------------------------------- paged cache, packed batches
+
+def _need(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _on(device, *tensors) -> None:
+    for t in tensors:
+        _need(t.is_cuda, "libgr_attn device entry points take device tensors")
+        _need(t.device == device, f"every tensor of a call lives on one device: {t.device} and {device}")
+
+
+def _ints(t, shape, name) -> None:
+    _need(t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous(),
+          f"{name} is a contiguous int32 tensor of shape {shape}")
+
+
+class _DeviceCall:
+    """A prepared call on tensors of one device; enqueued on `stream` (a stream of that
+    device) or on the device's current one."""
+
+    device: torch.device
+
+    def _enqueue(self, stream, fn, *args) -> None:
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        _need(stream.device == self.device, f"the call's tensors live on {self.device}, the stream on {stream.device}")
+        if torch.cuda.current_device() == self.device.index:
+            ffi.check(fn(*args, stream.cuda_stream))
+        else:
+            with torch.cuda.device(self.device):
+                ffi.check(fn(*args, stream.cuda_stream))
+
+
+class PagedCache:
+    """The K and V pages of one layer (gr_paged_cache).
+
+    k_pages / v_pages [n_pages][page_size][Hkv][d] (f16, bf16, or int8 Q8 codes), the same
+    strides, dims contiguous: a [n_pages][Hkv][page_size][d] buffer goes in as its
+    transpose(1, 2).  Q8: f32 k_scale / v_scale [n_pages][page_size][Hkv].
+    """
+
+    def __init__(self, k_pages, v_pages, k_scale=None, v_scale=None):
+        _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.dtype == v_pages.dtype
+              and k_pages.stride() == v_pages.stride() and k_pages.stride(3) == 1,
+              "k_pages and v_pages: [n_pages][page_size][n_kv_heads][head_dim] of one type and one set of strides, "
+              "dims contiguous")
+        _need(k_pages.dtype in (torch.float16, torch.bfloat16, torch.int8), "pages are f16, bf16 or int8")
+        self.device = k_pages.device
+        _on(self.device, k_pages, v_pages)
+        self._keep = (k_pages, v_pages, k_scale, v_scale)
+        c = ffi.PagedCacheDesc()
+        c.n_pages, c.page_size, c.n_kv_heads, c.head_dim = k_pages.shape
+        c.kv_dtype = _DT[k_pages.dtype]
+        c.k_pages, c.v_pages = _ptr(k_pages), _ptr(v_pages)
+        c.page_stride, c.row_stride, c.head_stride = _strides(k_pages, 3)
+        if k_pages.dtype == torch.int8:
+            _need(k_scale is not None and v_scale is not None, "Q8 pages need k_scale and v_scale")
+            _need(all(t.dtype == torch.float32 and t.shape == k_pages.shape[:3] for t in (k_scale, v_scale))
+                  and k_scale.stride() == v_scale.stride(),
+                  "k_scale and v_scale: f32 [n_pages][page_size][n_kv_heads] of one set of strides")
+            _on(self.device, k_scale, v_scale)
+            c.k_scale, c.v_scale = _ptr(k_scale), _ptr(v_scale)
+            c.scale_page_stride, c.scale_row_stride, c.scale_head_stride = _strides(k_scale, 3, 1)
+        else:
+            _need(k_scale is None and v_scale is None, "k_scale and v_scale belong to Q8 pages")
+        self.desc = c
+
+
+def _strides(t, n: int, least: int | None = None):
+    """The first n strides; that of a dimension of size 1 is never used and becomes a valid one."""
+    least = t.shape[-1] if least is None else least
+    return [least if t.shape[i] == 1 else s for i, s in enumerate(t.stride()[:n])]
+
+
+class PagedBatch:
+    """The rows of a step (gr_paged_batch): row_start int32 [n_seq + 1], kv_len int32
+    [n_seq], page_table int32 [n_seq][pages] (rows may be strided), all on the device and
+    read when a call's kernels run.  n_rows: rows of the step's row arrays; max_rows,
+    max_len: upper bounds of a sequence's rows and length."""
+
+    def __init__(self, row_start, kv_len, page_table, *, n_rows, max_rows, max_len):
+        _need(page_table.dim() == 2 and page_table.dtype == torch.int32
+              and (page_table.shape[1] == 1 or page_table.stride(1) == 1),
+              "page_table is an int32 tensor [n_seq][pages], pages contiguous")
+        n_seq, pages = page_table.shape
+        _ints(row_start, (n_seq + 1,), "row_start")
+        _ints(kv_len, (n_seq,), "kv_len")
+        self.device = row_start.device
+        _on(self.device, row_start, kv_len, page_table)
+        self._keep = (row_start, kv_len, page_table)
+        b = ffi.PagedBatchDesc()
+        b.n_seq, b.n_rows, b.max_rows, b.max_len = n_seq, int(n_rows), int(max_rows), int(max_len)
+        b.row_start, b.kv_len, b.page_table = _ptr(row_start), _ptr(kv_len), _ptr(page_table)
+        b.table_stride, b.table_pages = max(page_table.stride(0), pages) if n_seq == 1 else page_table.stride(0), pages
+        self.desc = b
+
+
+class _PagedKvCall(_DeviceCall):
+    _fn = ""
+
+    def __init__(self, cache: PagedCache, batch: PagedBatch, k, v):
+        _need(k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype and k.stride() == v.stride()
+              and k.stride(2) == 1, "k and v: rows [n_rows][n_kv_heads][head_dim] of one type and one set of strides")
+        _need(k.dtype in (torch.float32, torch.float16, torch.bfloat16), "rows are f32, f16 or bf16")
+        c, b = cache.desc, batch.desc
+        _need(tuple(k.shape) == (b.n_rows, c.n_kv_heads, c.head_dim),
+              f"rows of shape {tuple(k.shape)}: the batch and the cache say {(b.n_rows, c.n_kv_heads, c.head_dim)}")
+        self.device = cache.device
+        _on(self.device, k, v, batch._keep[0])
+        r = ffi.PagedRows()
+        r.dtype, r.k, r.v = _DT[k.dtype], _ptr(k), _ptr(v)
+        r.row_stride, r.head_stride = _strides(k, 2)
+        self._keep = (cache, batch, k, v)
+        self.args = r
+        self._call = (getattr(ffi.lib(), self._fn), ctypes.byref(c), ctypes.byref(b), ctypes.byref(r))
+
+    def __call__(self, stream=None) -> None:
+        self._enqueue(stream, *self._call)
+
+
+class PagedWriteCall(_PagedKvCall):
+    """A prepared gr_paged_kv_write: the batch's K / V rows [n_rows][Hkv][d] (f32, f16 or
+    bf16) go to their pages, rounded or quantised to the cache's type."""
+
+    _fn = "gr_paged_kv_write"
+
+
+class PagedReadCall(_PagedKvCall):
+    """A prepared gr_paged_kv_read: the batch's positions read out of their pages into k and
+    v [n_rows][Hkv][d] (f32, f16 or bf16)."""
+
+    _fn = "gr_paged_kv_read"
+
+
+def _check_qo(q, out) -> None:
+    _need(q.dim() == 3 and out.shape == q.shape and out.dtype == q.dtype and q.stride(2) == 1 and out.stride(2) == 1,
+          "q and out: rows [n_rows][n_heads][head_dim] of one type, dims contiguous")
+    _need(q.dtype in (torch.float16, torch.bfloat16), "q and out are f16 or bf16")
+
+
+class PagedAttentionCall(_DeviceCall):
+    """A prepared gr_paged_attention (args + workspace): q / out [n_rows][Hq][d] (f16 or bf16,
+    the pages' type unless they are Q8); the pages hold the batch's rows already.  Calls that
+    may overlap (other streams, graphs replayed side by side) are prepared separately: each
+    has its own workspace."""
+
+    def __init__(self, cache: PagedCache, batch: PagedBatch, q, out, *, window=0, score_scale=None):
+        _check_qo(q, out)
+        c, b = cache.desc, batch.desc
+        _need(q.shape[0] == b.n_rows and q.shape[2] == c.head_dim,
+              f"q of shape {tuple(q.shape)}: the batch has {b.n_rows} rows, the cache head_dim {c.head_dim}")
+        self.device = cache.device
+        _on(self.device, q, out, batch._keep[0])
+        a = ffi.PagedAttentionArgs()
+        a.n_heads, a.dtype, a.window = q.shape[1], _DT[q.dtype], int(window)
+        a.score_scale = 1.0 / math.sqrt(c.head_dim) if score_scale is None else float(score_scale)
+        a.q, a.out = _ptr(q), _ptr(out)
+        a.q_row_stride, a.q_head_stride = _strides(q, 2)
+        a.out_row_stride, a.out_head_stride = _strides(out, 2)
+        args = (ctypes.byref(c), ctypes.byref(b), ctypes.byref(a))
+        self.ws = _workspace(ffi.lib().gr_paged_attention_workspace_size(*args), self.device)
+        a.workspace = _aligned(self.ws)
+        self._keep = (cache, batch, q, out)
+        self.args = a
+        self._call = (ffi.lib().gr_paged_attention, *args)
+
+    def __call__(self, stream=None) -> None:
+        self._enqueue(stream, *self._call)
+
+
+def paged_attention(cache: PagedCache, batch: PagedBatch, q, *, out=None, window=0, score_scale=None):
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)  # rows of no sequence stay zero
+    PagedAttentionCall(cache, batch, q, out, window=window, score_scale=score_scale)()
+    return out
+
+
+class PackedAttentionCall(_DeviceCall):
+    """A prepared gr_packed_attention (args + workspace): causal attention inside each of the
+    prompts that lie one after another in q [n_rows][Hq][d], k and v [n_rows][Hkv][d] (f16
+    or bf16); seq_start int32 [n_seq + 1]; out as q; max_rows an upper bound of the longest
+    prompt.  Calls that may overlap are prepared separately, as PagedAttentionCall."""
+
+    def __init__(self, q, k, v, seq_start, out, *, max_rows, window=0, score_scale=None):
+        _check_qo(q, out)
+        n_rows, n_heads, d = q.shape
+        _need(k.dim() == 3 and k.shape == v.shape and k.stride() == v.stride() and k.stride(2) == 1
+              and k.dtype == v.dtype == q.dtype and k.shape[0] == n_rows and k.shape[2] == d,
+              "k and v: rows [n_rows][n_kv_heads][head_dim] of q's type and of one set of strides")
+        _need(seq_start.dim() == 1 and seq_start.numel() >= 1, "seq_start has n_seq + 1 entries")
+        _ints(seq_start, (seq_start.numel(),), "seq_start")
+        self.device = q.device
+        _on(self.device, q, k, v, seq_start, out)
+        a = ffi.PackedArgs()
+        a.n_seq, a.n_rows, a.max_rows = seq_start.numel() - 1, n_rows, int(max_rows)
+        a.n_heads, a.n_kv_heads, a.head_dim, a.dtype = n_heads, k.shape[1], d, _DT[q.dtype]
+        a.window = int(window)
+        a.score_scale = 1.0 / math.sqrt(d) if score_scale is None else float(score_scale)
+        a.seq_start, a.q, a.k, a.v, a.out = _ptr(seq_start), _ptr(q), _ptr(k), _ptr(v), _ptr(out)
+        a.q_row_stride, a.q_head_stride = _strides(q, 2)
+        a.kv_row_stride, a.kv_head_stride = _strides(k, 2)
+        a.out_row_stride, a.out_head_stride = _strides(out, 2)
+        self.ws = _workspace(ffi.lib().gr_packed_attention_workspace_size(ctypes.byref(a)), self.device)
+        a.workspace = _aligned(self.ws)
+        self._keep = (q, k, v, seq_start, out)
+        self.args = a
+
+    def __call__(self, stream=None) -> None:
+        self._enqueue(stream, ffi.lib().gr_packed_attention, ctypes.byref(self.args))
+
+
+def packed_attention(q, k, v, seq_start, *, max_rows, out=None, window=0, score_scale=None):
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)  # rows of no prompt stay zero
+    PackedAttentionCall(q, k, v, seq_start, out, max_rows=max_rows, window=window, score_scale=score_scale)()
+    return out
