@@ -1,0 +1,13 @@
+// head_dim 128 of the attention over pages and packed rows (paged_attn.hpp).
+#include <algorithm>
+
+#include "paged_attn.hpp"
+
+namespace gr {
+
+using K128 = PaKernels<PaTile<128, 1, 4, 128, 1>, PaTile<128, 4, 1, 64, 2>, PaTile<128, 8, 1, 128, 2>>;
+
+size_t paged_attn_ws_d128(const PagedAttnLaunch& p) { return K128::ws(p); }
+hipError_t launch_paged_attn_d128(const PagedAttnLaunch& p, hipStream_t st) { return K128::launch_any(p, st); }
+
+}  // namespace gr

@@ -1,0 +1,13 @@
+// head_dim 256 of the attention over pages and packed rows (paged_attn.hpp).
+#include <algorithm>
+
+#include "paged_attn.hpp"
+
+namespace gr {
+
+using K256 = PaKernels<PaTile<256, 1, 2, 64, 1>, PaTile<256, 4, 1, 64, 1>, PaTile<256, 4, 1, 64, 1>>;
+
+size_t paged_attn_ws_d256(const PagedAttnLaunch& p) { return K256::ws(p); }
+hipError_t launch_paged_attn_d256(const PagedAttnLaunch& p, hipStream_t st) { return K256::launch_any(p, st); }
+
+}  // namespace gr

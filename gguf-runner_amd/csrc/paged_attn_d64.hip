@@ -1,0 +1,13 @@
+// head_dim 64 of the attention over pages and packed rows (paged_attn.hpp).
+#include <algorithm>
+
+#include "paged_attn.hpp"
+
+namespace gr {
+
+using K64 = PaKernels<PaTile<64, 1, 4, 128, 2>, PaTile<64, 4, 1, 128, 2>, PaTile<64, 8, 1, 128, 4>>;
+
+size_t paged_attn_ws_d64(const PagedAttnLaunch& p) { return K64::ws(p); }
+hipError_t launch_paged_attn_d64(const PagedAttnLaunch& p, hipStream_t st) { return K64::launch_any(p, st); }
+
+}  // namespace gr

@@ -62,6 +62,9 @@ __device__ __forceinline__ PagedPlace pk_place(const PagedSeqs& s, int row, int 
     return at;
 }
 
+// Head rows below this magnitude (2^-100) store as zeros: their scale would leave f32's normal range.
+constexpr float kQ8Least = 7.8886091e-31f;
+
 // code of x: round(x * inv) with halves away from zero, as quantize_row_q8
 // (inference.rs:249-268); a NaN becomes 0, as Rust's saturating `as i8`.
 __device__ __forceinline__ uint32_t pk_code(float x, float inv) {
@@ -110,7 +113,8 @@ __global__ __launch_bounds__(kPagedKvThreads) void paged_kv_kernel(const PagedKv
                 // a head's CPH pieces are CPH adjacent lanes (lanes_per_row is a multiple of CPH)
 #pragma unroll
                 for (int m = CPH / 2; m >= 1; m >>= 1) amax = fmaxf(amax, shfl_xor(amax, m));
-                const float inv = amax == 0.0f ? 0.0f : __fdiv_rn(127.0f, amax);
+                if (amax < kQ8Least) amax = 0.0f;
+                const float inv = amax == 0.0f ? 0.0f : __fdiv_rn(1.0f, amax) * 127.0f;
                 uint32_t w0 = 0, w1 = 0;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -119,7 +123,7 @@ __global__ __launch_bounds__(kPagedKvThreads) void paged_kv_kernel(const PagedKv
                 }
                 *(uint2*)((int8_t*)p.pages[which] + e) = make_uint2(w0, w1);
                 if (i == 0)
-                    p.scale[which][sc0 + g * p.scale_head_stride] = amax == 0.0f ? 1.0f : __fdiv_rn(amax, 127.0f);
+                    p.scale[which][sc0 + g * p.scale_head_stride] = amax == 0.0f ? 1.0f : amax * (1.0f / 127.0f);
             } else {
                 pk_store8<KV>((typename KV::storage*)p.pages[which] + e, x);
             }

@@ -83,9 +83,11 @@ typedef struct gr_paged_rows {
 } gr_paged_rows;
 
 /* Store the batch's rows in their pages.  16-bit pages: rounded to nearest even.  Q8
- * pages: per (row, head), amax = max |x|; scale = amax / 127 (1 when amax is 0); code =
- * clamp(round(x * (127 / amax)), -127, 127), halves away from zero, every step rounded
- * to f32 (quantize_row_q8 over one head's row).  A row whose page id names no page is
+ * pages: per (row, head), amax = max |x|; scale = amax * (1/127); code = clamp(round(x *
+ * (127 * (1/amax))), -127, 127), halves away from zero, every quotient and product
+ * rounded to f32 (quantize_row_q8 over one head's row, with reciprocals); an amax below
+ * 2^-100 counts as 0: scale 1, codes 0.  A NaN stores as 0; an infinity makes its head
+ * row read as NaN. A row whose page id names no page is
  * dropped.  Sequences may share pages they only read; no two rows of a call may name
  * the same place. */
 int gr_paged_kv_write(const gr_paged_cache* c, const gr_paged_batch* b, const gr_paged_rows* rows, void* stream);

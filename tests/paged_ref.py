@@ -12,13 +12,14 @@ HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat1
 
 
 def quantise(x):
-    """Q8 codes and scales of f32 rows [..][d] (quantize_row_q8 per head row), in numpy so
-    that every step is one f32 rounding."""
+    """Q8 codes and scales of f32 rows [..][d], in numpy so that every step is one f32
+    rounding: scale = amax * (1/127), code = round(x * (127 * (1/amax)))."""
     x = x.detach().float().cpu().numpy()
+    one, top = np.float32(1), np.float32(127)
     amax = np.abs(x).max(-1, keepdims=True)
-    with np.errstate(divide="ignore", over="ignore"):
-        scale = np.where(amax == 0, np.float32(1), amax / np.float32(127)).astype(np.float32)
-        inv = np.where(amax == 0, np.float32(0), np.float32(127) / np.where(amax == 0, np.float32(1), amax))
+    amax = np.where(amax < np.float32(2.0 ** -100), np.float32(0), amax)
+    scale = np.where(amax == 0, one, amax * (one / top)).astype(np.float32)
+    inv = np.where(amax == 0, np.float32(0), one / np.where(amax == 0, one, amax) * top)
     y = (x * inv.astype(np.float32)).astype(np.float32)
     whole = np.trunc(y)
     y = whole + np.where(np.abs(y - whole) >= 0.5, np.sign(y), 0)
