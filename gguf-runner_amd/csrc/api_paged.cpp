@@ -138,6 +138,12 @@ int check_qo(const char* fn, const void* q, const void* out, int head_dim, int64
     return GR_OK;
 }
 
+int check_fits(const char* fn, const PagedAttnLaunch& p) {
+    if (!paged_attn_fits(p))
+        return fail(GR_ERR_ARG, "%s: rows, sequences and positions beyond 2^31 tiles of work: divide the batch", fn);
+    return GR_OK;
+}
+
 int check_ws(const char* fn, const void* ws) {
     if (!ws) return fail(GR_ERR_ARG, "%s: null workspace", fn);
     if ((uintptr_t)ws % 256) return fail(GR_ERR_ARG, "%s: workspace must be 256-byte aligned", fn);
@@ -176,7 +182,7 @@ int paged_attn_args(const char* fn, const gr_paged_cache* c, const gr_paged_batc
     p->scale_head_stride = c->scale_head_stride;
     p->max_rows = b->max_rows, p->max_len = b->max_len;
     p->workspace = a->workspace;
-    return GR_OK;
+    return check_fits(fn, *p);
 }
 
 int packed_args(const char* fn, const gr_packed_args* a, PagedAttnLaunch* p, bool* none) {
@@ -220,7 +226,7 @@ int packed_args(const char* fn, const gr_packed_args* a, PagedAttnLaunch* p, boo
     p->row_stride = a->kv_row_stride, p->head_stride = a->kv_head_stride;
     p->max_rows = a->max_rows, p->max_len = a->max_rows;
     p->workspace = a->workspace;
-    return GR_OK;
+    return check_fits(fn, *p);
 }
 
 }  // namespace

@@ -5,6 +5,10 @@
 
 namespace gr {
 
+bool paged_attn_fits(const PagedAttnLaunch& p) {
+    return p.head_dim == 64 ? paged_attn_fits_d64(p) : p.head_dim == 128 ? paged_attn_fits_d128(p) : paged_attn_fits_d256(p);
+}
+
 size_t paged_attn_ws_bytes(const PagedAttnLaunch& p) {
     return p.head_dim == 64 ? paged_attn_ws_d64(p) : p.head_dim == 128 ? paged_attn_ws_d128(p) : paged_attn_ws_d256(p);
 }

@@ -75,10 +75,11 @@ struct PaMat<BF16> {
 
 enum PaSrc { kPaPacked = 0, kPaPages = 1, kPaPagesQ8 = 2 };
 
-// Tiles of a kernel: RW row groups x KH key parts, BN keys, waves per SIMD it is built for.
-template <int D_, int RW_, int KH_, int BN_, int OCC_>
+// Tiles of a kernel: RW row groups x KH key parts, BN keys, NBUF tiles in LDS (NBUF - 1 of
+// them on their way), waves per SIMD it is built for.
+template <int D_, int RW_, int KH_, int BN_, int NBUF_, int OCC_>
 struct PaTile {
-    static constexpr int D = D_, RW = RW_, KH = KH_, BN = BN_, OCC = OCC_;
+    static constexpr int D = D_, RW = RW_, KH = KH_, BN = BN_, NBUF = NBUF_, OCC = OCC_;
     static constexpr int NW = RW * KH, NT = NW * 64, BM = RW * 32;
     static_assert(BN % (32 * KH) == 0, "every key part has its sub-tiles");
 };
@@ -98,7 +99,12 @@ __device__ __forceinline__ uint4 pa_load16(__amdgpu_buffer_rsrc_t r, int voff) {
     return uint4{};
 #endif
 }
-__device__ __forceinline__ void pa_wait_vmem() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+// s_waitcnt vmcnt(N): all but the last N vector memory operations of the wave are done
+template <int N>
+__device__ __forceinline__ void pa_wait_vmem() {
+    static_assert(N < 64, "vmcnt has 6 bits");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
+}
 __device__ __forceinline__ float pa_xmax32(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -135,115 +141,155 @@ constexpr float kPaLeastScale = 7.8886091e-31f;  // 2^-100: smaller v_scales cou
 
 // ---------------------------------------------------------------- schedules
 
-// One block's place: rows [row0, row0 + n_pr) packed, keys.
+// What a sequence has: rows, keys, blocks, and the tiles that each of its blocks counts in
+// the stream (its longest block's, at least 1).  0 blocks behind the last sequence.
+struct PaSeq {
+    int beg, n, len, nb, vt;
+};
+template <int BM, int BN>
+__device__ __forceinline__ PaSeq pa_seq(const PagedAttnLaunch& p, int s) {
+    PaSeq r{0, 0, 0, 0, 0};
+    if (s >= p.seqs.n_seq) return r;
+    const int group = p.n_heads / p.n_kv_heads;
+    r.beg = seq_row(p.seqs, s);
+    r.n = max(seq_row(p.seqs, s + 1) - r.beg, 0);
+    r.len = seq_len(p.seqs, s, r.n);
+    r.nb = (r.n * group + BM - 1) / BM;
+    r.vt = (r.len + BN - 1) / BN;
+    if (p.window > 0) r.vt = min(r.vt, (min(p.window, r.len) + BM / group + BN - 1) / BN + 1);
+    r.vt = max(r.vt, 1);
+    return r;
+}
+
+// Inclusive sum over the wave's lanes: four shifts inside rows of 16 lanes, then each row's
+// last lane is added to the rows behind it.
+__device__ __forceinline__ int pa_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
+    return x;
+}
+__device__ __forceinline__ int pa_last(int x) { return __builtin_amdgcn_readlane(x, 63); }
+
+// One block: KV head g, block rb of sequence seq, its rows and keys.
 struct PaBlock {
     int seq, rb, g;
-    int beg, n, p0;      // first row, rows, position of the first row
-    int t_first, kend;   // keys [.., kend), tiles start at t_first
+    int beg, n, p0;           // first row, rows, position of the first row
+    int nb, vt;
+    int t_first, kend;        // keys [.., kend); tiles start at t_first
     int n_tiles;
 };
-
 template <int BM, int BN>
-__device__ __forceinline__ void pa_block(const PagedAttnLaunch& p, PaBlock& b) {
+__device__ __forceinline__ void pa_keys(const PagedAttnLaunch& p, PaBlock& b) {
     const int group = p.n_heads / p.n_kv_heads;
-    b.beg = seq_row(p.seqs, b.seq);
-    b.n = seq_row(p.seqs, b.seq + 1) - b.beg;
-    const int len = seq_len(p.seqs, b.seq, b.n);
-    b.p0 = len - b.n;
     const int tok0 = b.rb * BM / group, tok1 = (min((b.rb + 1) * BM, b.n * group) - 1) / group;
     b.kend = max(b.p0 + tok1 + 1, 0);
     const int lo = p.window > 0 ? max(b.p0 + tok0 + 1 - p.window, 0) : 0;
     b.t_first = lo / BN * BN;
     b.n_tiles = b.kend > b.t_first ? (b.kend - b.t_first + BN - 1) / BN : 0;
 }
-
-// Blocks of sequence s and the tiles that each of them counts in the stream (at least its
-// longest one's, so that the cuts fall evenly: 1 for a sequence of no keys).
-template <int BM, int BN>
-__device__ __forceinline__ void pa_counts(const PagedAttnLaunch& p, int s, int& nb, int& vt) {
-    nb = vt = 0;
-    if (s >= p.seqs.n_seq) return;
-    const int group = p.n_heads / p.n_kv_heads;
-    const int n = max(seq_row(p.seqs, s + 1) - seq_row(p.seqs, s), 0);
-    nb = (n * group + BM - 1) / BM;
-    const int len = seq_len(p.seqs, s, n);
-    vt = (len + BN - 1) / BN;
-    if (p.window > 0) {
-        const int64_t most = ((int64_t)p.window + (BM + group - 1) / group + BN - 1) / BN + 1;
-        if (vt > most) vt = (int)most;
-    }
-    vt = max(vt, 1);
+__device__ __forceinline__ void pa_take(PaBlock& b, const PaSeq& c, int s0, int l) {
+    b.seq = s0 + l;
+    b.beg = __builtin_amdgcn_readlane(c.beg, l);
+    b.n = __builtin_amdgcn_readlane(c.n, l);
+    b.p0 = __builtin_amdgcn_readlane(c.len, l) - b.n;
+    b.nb = __builtin_amdgcn_readlane(c.nb, l);
+    b.vt = __builtin_amdgcn_readlane(c.vt, l);
 }
 
-__device__ __forceinline__ int64_t pa_scan(int64_t x) {  // inclusive, over the wave
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-    }
-    return x;
-}
-
-// The stream: sequence s takes cost(s) = n_kv_heads * nb(s) * vt(s) places, in that order.
+// The stream: sequence s takes n_kv_heads * nb * vt places (the host bounds their sum by
+// 2^31), KV head by KV head, block by block; place v of a block is its tile v.
 template <int BM, int BN>
-__device__ __forceinline__ int64_t pa_stream_total(const PagedAttnLaunch& p) {
-    int64_t t = 0;
-    for (int s0 = 0; s0 < p.seqs.n_seq; s0 += 64) {
-        int nb, vt;
-        pa_counts<BM, BN>(p, s0 + (threadIdx.x & 63), nb, vt);
-        t += __shfl(pa_scan((int64_t)nb * vt * p.n_kv_heads), 63, 64);
+__device__ __forceinline__ int pa_stream_total(const PagedAttnLaunch& p, const PaSeq& c0) {
+    int t = pa_last(pa_scan(c0.nb * c0.vt * p.n_kv_heads));
+    for (int s0 = 64; s0 < p.seqs.n_seq; s0 += 64) {
+        const PaSeq c = pa_seq<BM, BN>(p, s0 + (threadIdx.x & 63));
+        t += pa_last(pa_scan(c.nb * c.vt * p.n_kv_heads));
     }
     return t;
 }
-
-// Where place x (< total) of the stream is: block, its vt and x's offset in it.
-struct PaPlace {
-    int seq, rb, g, vt;
-    int64_t at;
-};
+// The block that place x (< total) belongs to; returns x's offset in it.  c0: pa_seq of the lane.
 template <int BM, int BN>
-__device__ __forceinline__ PaPlace pa_stream_find(const PagedAttnLaunch& p, int64_t x) {
-    PaPlace r{0, 0, 0, 1, 0};
+__device__ __forceinline__ int pa_stream_find(const PagedAttnLaunch& p, const PaSeq& c0, int x, PaBlock& b) {
     for (int s0 = 0; s0 < p.seqs.n_seq; s0 += 64) {
-        int nb, vt;
-        pa_counts<BM, BN>(p, s0 + (threadIdx.x & 63), nb, vt);
-        const int64_t cost = (int64_t)nb * vt * p.n_kv_heads;
-        const int64_t incl = pa_scan(cost);
-        const int64_t all = __shfl(incl, 63, 64);
+        const PaSeq c = s0 == 0 ? c0 : pa_seq<BM, BN>(p, s0 + (threadIdx.x & 63));
+        const int cost = c.nb * c.vt * p.n_kv_heads;
+        const int incl = pa_scan(cost);
+        const int all = pa_last(incl);
         if (x < all) {
             const int l = __ffsll((unsigned long long)__ballot(x < incl)) - 1;
-            const int64_t in = x - __shfl(incl - cost, l, 64);
-            r.seq = __builtin_amdgcn_readfirstlane(s0 + l);
-            nb = __builtin_amdgcn_readfirstlane(__shfl(nb, l, 64));
-            r.vt = __builtin_amdgcn_readfirstlane(__shfl(vt, l, 64));
-            const int64_t blk = in / r.vt;
-            r.at = in - blk * r.vt;
-            r.g = __builtin_amdgcn_readfirstlane((int)(blk / nb));
-            r.rb = __builtin_amdgcn_readfirstlane((int)(blk - (int64_t)r.g * nb));
-            break;
+            x -= __builtin_amdgcn_readlane(incl - cost, l);
+            pa_take(b, c, s0, l);
+            const int i = x / b.vt;
+            b.g = i / b.nb;
+            b.rb = i - b.g * b.nb;
+            pa_keys<BM, BN>(p, b);
+            return x - i * b.vt;
         }
         x -= all;
     }
-    return r;
+    return 0;
 }
 
 // Workgroup b of a stream launch as a place among them: XCD b % 8 gets a run of
 // neighbouring ranges (the blocks of a sequence's KV head share its tiles in one L2).
-__device__ __forceinline__ int pa_stream_rank(int b, int g) {
-    const int per = g / 8;  // workgroups of a launch: a multiple of 8
-    return (b & 7) * per + (b >> 3);
+// Launches are multiples of 8 workgroups.
+__device__ __forceinline__ int pa_stream_rank(int b, int n) { return (b & 7) * (n / 8) + (b >> 3); }
+// Places per range: an equal share, at least least.
+__device__ __forceinline__ int pa_stream_q(int total, int n, int least) {
+    return max((int)(((int64_t)total + n - 1) / n), least);
 }
-__device__ __forceinline__ int64_t pa_stream_q(int64_t total, int g) { return (total + g - 1) / g; }
 
-// The real tiles [a, b) of a block of n_tiles for virtual ones [va, vb) of vt.
-__device__ __forceinline__ int pa_real(int64_t v, int n_tiles, int vt) { return (int)(v * n_tiles / vt); }
+// ORDERED: item idx of one KV head, longest blocks first: blocks by their number counted
+// from a sequence's first, the highest numbers first (up to 64 sequences); more sequences:
+// one after another, each one's last block first.  False: no such item.
+template <int BM, int BN>
+__device__ __forceinline__ bool pa_ordered_find(const PagedAttnLaunch& p, const PaSeq& c0, int idx, PaBlock& b) {
+    const int lane = threadIdx.x & 63;
+    if (p.seqs.n_seq <= 64) {
+        auto count = [&](int l) { return pa_last(pa_scan(max(c0.nb - l, 0))); };  // blocks numbered l or more
+        if (idx >= count(0)) return false;
+        int lo = 0, hi = 1;  // lo: the highest l with count(l) > idx
+        while (count(hi) > idx) hi *= 2;
+        while (hi - lo > 1) {
+            const int mid = lo + (hi - lo) / 2;
+            if (count(mid) > idx) lo = mid;
+            else hi = mid;
+        }
+        const int k = idx - count(lo + 1);  // the k-th sequence that has a block of this number
+        const bool has = c0.nb > lo;
+        const int before = __popcll(__ballot(has) & ((1ull << lane) - 1));
+        const int l = __ffsll((unsigned long long)__ballot(has && before == k)) - 1;
+        pa_take(b, c0, 0, l);
+        b.rb = lo;
+    } else {
+        int s0 = 0;
+        for (;; s0 += 64) {
+            if (s0 >= p.seqs.n_seq) return false;
+            const PaSeq c = s0 == 0 ? c0 : pa_seq<BM, BN>(p, s0 + lane);
+            const int incl = pa_scan(c.nb);
+            const int all = pa_last(incl);
+            if (idx < all) {
+                const int l = __ffsll((unsigned long long)__ballot(idx < incl)) - 1;
+                pa_take(b, c, s0, l);
+                b.rb = __builtin_amdgcn_readlane(incl, l) - 1 - idx;
+                break;
+            }
+            idx -= all;
+        }
+    }
+    pa_keys<BM, BN>(p, b);
+    return true;
+}
 
 // ---------------------------------------------------------------- the kernel
 
 template <typename DT, typename T, int SRC, bool STREAM>
 __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAttnLaunch p) {
-    constexpr int D = T::D, BN = T::BN, BM = T::BM, RW = T::RW, KH = T::KH, NT = T::NT;
+    constexpr int D = T::D, BN = T::BN, BM = T::BM, RW = T::RW, KH = T::KH, NT = T::NT, NBUF = T::NBUF;
     constexpr bool kQ8 = SRC == kPaPagesQ8;
     using M = PaMat<DT>;
     constexpr int CPR = D / 8;              // 16-byte chunks per tile row
@@ -253,30 +299,39 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     constexpr int RPV = 64 / SCPR;          // ... of a wave: inside one run of 16 rows, so one page
     constexpr int EB = kQ8 ? 1 : 2;         // bytes per stored element
     static_assert(LD >= 1 && LD <= 32 && BN * SCPR % NT == 0 && BN / 16 <= 32 && BN <= NT, "tile shape");
+    static_assert(NBUF == 2 || (NBUF == 4 && !kQ8), "buffers");
 
+    // distinct arrays, so that the compiler sees that filling one never aliases reading another
     __shared__ __attribute__((aligned(16))) uint16_t Ks0[BN * D];
     __shared__ __attribute__((aligned(16))) uint16_t Ks1[BN * D];
     __shared__ __attribute__((aligned(16))) uint16_t Vs0[BN * D];
     __shared__ __attribute__((aligned(16))) uint16_t Vs1[BN * D];
+    __shared__ __attribute__((aligned(16))) uint16_t Ks2[NBUF == 4 ? BN * D : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t Ks3[NBUF == 4 ? BN * D : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t Vs2[NBUF == 4 ? BN * D : 8];
+    __shared__ __attribute__((aligned(16))) uint16_t Vs3[NBUF == 4 ? BN * D : 8];
     // Q8: c * k_scale, log2 v_scale, 1 / v_scale of the tile's keys
     __shared__ __attribute__((aligned(16))) float Sc0[kQ8 ? 3 * BN : 4];
     __shared__ __attribute__((aligned(16))) float Sc1[kQ8 ? 3 * BN : 4];
+    // Page ids of a run of tiles (-1: not there): read from the table once per run, so that
+    // no load of a tile waits for another
+    constexpr int kIds = 512;
+    __shared__ int Ids[SRC == kPaPacked ? 1 : kIds];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = KH > 1 ? wave % RW : wave, kh = KH > 1 ? wave / RW : 0;
     const int ln = lane & 31, lg = lane >> 5;
     const int group = p.n_heads / p.n_kv_heads;
-    const int ps1 = (1 << p.seqs.page_shift) - 1;
+    const int shift = p.seqs.page_shift;
+    const int ps1 = (1 << shift) - 1;
 
     // this thread's source chunks: row wave * RPV + lane / SCPR + u * RPU of the tile
     const int lrow = lane / SCPR;
-    int col[LD];  // byte offset in the source row
-#pragma unroll
-    for (int u = 0; u < LD; u++) {
-        const int r = wave * RPV + lrow + u * RPU;
-        col[u] = kQ8 ? lane % SCPR * 16 : ((lane % SCPR) ^ pa_swz<D>(r & 15)) * 16;
-    }
+    auto col = [&](int u) {  // byte offset in the source row
+        const int r = wave * RPV + lrow + (RPU % 16 ? u * RPU : 0);
+        return kQ8 ? lane % SCPR * 16 : ((lane % SCPR) ^ pa_swz<D>(r & 15)) * 16;
+    };
     const int rsb = (int)p.row_stride * EB;
     const int swz_k = pa_swz<D>(ln & 15);
     const int gi = lane & 15;
@@ -290,16 +345,15 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     }
 
     // ------------------------------------------------ the workgroup's range
-    int64_t pos = 0, stop = 1;  // STREAM: places of the stream
-    int64_t total = 0, q_len = 0;
-    int rank = 0;
-    PaPlace pl{};
+    const PaSeq c0 = pa_seq<BM, BN>(p, lane);
+    int pos = 0, stop = 1, rank = 0;  // STREAM: places of the stream
     if constexpr (STREAM) {
-        total = pa_stream_total<BM, BN>(p);
+        const int total = pa_stream_total<BM, BN>(p, c0);
         rank = pa_stream_rank(blockIdx.x, gridDim.x);
-        q_len = pa_stream_q(total, gridDim.x);
-        pos = rank * q_len;
-        stop = min(total, pos + q_len);
+        const int q = pa_stream_q(total, gridDim.x, p.least);
+        if ((int64_t)rank * q >= total) return;
+        pos = rank * q;
+        stop = min((int64_t)total, (int64_t)pos + q);
     }
 
     while (pos < stop) {
@@ -308,88 +362,39 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         bool whole = true;
         int slot = 0;
         if constexpr (STREAM) {
-            pl = pa_stream_find<BM, BN>(p, pos);
-            blk.seq = pl.seq, blk.rb = pl.rb, blk.g = pl.g;
-            pa_block<BM, BN>(p, blk);
-            const int64_t vb = min((int64_t)pl.vt, pl.at + (stop - pos));
-            whole = pl.at == 0 && vb == pl.vt;
-            slot = 2 * rank + (pl.at == 0 ? 1 : 0);
-            it0 = pa_real(pl.at, blk.n_tiles, pl.vt);
-            it1 = pa_real(vb, blk.n_tiles, pl.vt);
-            pos += vb - pl.at;
+            const int at = pa_stream_find<BM, BN>(p, c0, pos, blk);
+            const int to = min(blk.vt, at + (stop - pos));
+            whole = at == 0 && to == blk.vt;
+            slot = 2 * rank + (at == 0 ? 1 : 0);
+            it0 = min(at, blk.n_tiles);
+            it1 = min(to, blk.n_tiles);
+            pos += to - at;
             if (!whole && it0 == it1) continue;  // the joining kernel knows that this piece is empty
         } else {
             pos = 1;
-            // the item's place in the order
             const int hx = p.n_kv_heads;
-            int idx, g;
             const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
+            int idx;
             if (8 % hx == 0) {  // 8 / hx XCDs take the blocks of one KV head
-                g = x % hx;
+                blk.g = x % hx;
                 idx = i * (8 / hx) + x / hx;
             } else if (hx % 8 == 0) {
-                g = x + 8 * (i % (hx / 8));
+                blk.g = x + 8 * (i % (hx / 8));
                 idx = i / (hx / 8);
             } else {
-                g = blockIdx.x % hx;
+                blk.g = blockIdx.x % hx;
                 idx = blockIdx.x / hx;
             }
-            int seq = -1, rb = 0;
-            if (p.seqs.n_seq <= 64) {
-                // longest first: blocks by their number from the highest, C(l) = blocks numbered l or more
-                int nb, vt;
-                pa_counts<BM, BN>(p, lane, nb, vt);
-                auto count = [&](int l) {
-                    int c = max(nb - l, 0);
-#pragma unroll
-                    for (int m = 32; m >= 1; m >>= 1) c += __shfl_xor(c, m, 64);
-                    return __builtin_amdgcn_readfirstlane(c);
-                };
-                if (idx >= count(0)) return;
-                int lo = 0, hi = 1;  // the highest l with C(l) > idx
-                while (count(hi) > idx) hi *= 2;
-                while (hi - lo > 1) {
-                    const int mid = lo + (hi - lo) / 2;
-                    if (count(mid) > idx) lo = mid;
-                    else hi = mid;
-                }
-                rb = lo;
-                int k = idx - count(lo + 1);  // the k-th sequence with a block of this number
-                const uint64_t has = __ballot(nb > lo);
-                const int before = __popcll(has & ((1ull << lane) - 1));
-                seq = __ffsll((unsigned long long)__ballot(nb > lo && before == k)) - 1;
-            } else {
-                for (int s0 = 0; s0 < p.seqs.n_seq; s0 += 64) {
-                    int nb, vt;
-                    pa_counts<BM, BN>(p, s0 + lane, nb, vt);
-                    const int incl = (int)pa_scan(nb);
-                    const int all = __builtin_amdgcn_readfirstlane(__shfl(incl, 63, 64));
-                    if (idx < all) {
-                        const int l = __ffsll((unsigned long long)__ballot(idx < incl)) - 1;
-                        seq = s0 + l;
-                        rb = __builtin_amdgcn_readfirstlane(__shfl(incl, l, 64)) - 1 - idx;  // its last block first
-                        break;
-                    }
-                    idx -= all;
-                }
-                if (seq < 0) return;
-            }
-            blk.seq = __builtin_amdgcn_readfirstlane(seq);
-            blk.rb = rb;
-            blk.g = g;
-            pa_block<BM, BN>(p, blk);
+            if (!pa_ordered_find<BM, BN>(p, c0, idx, blk)) return;
             it1 = blk.n_tiles;
         }
 
         const int n_pr = blk.n * group;
-        const int r0 = blk.rb * BM;
-        const int wr0 = r0 + rw * 32;
+        const int wr0 = blk.rb * BM + rw * 32;
         const bool wave_active = wr0 < n_pr;
-        const int my_row = wr0 + ln;
-        const bool row_ok = my_row < n_pr;
-        const int row_c = min(my_row, n_pr - 1);
-        const int my_tok = row_c / group;
-        const int my_h = blk.g * group + (row_c - my_tok * group);
+        // the lane's row, its token and position
+        auto token_of = [&](int r) { return min(r, n_pr - 1) / group; };
+        const int my_tok = token_of(wr0 + ln);
         const int my_pos = blk.p0 + my_tok;
         const int my_lo = p.window > 0 ? max(my_pos + 1 - p.window, 0) : 0;
         const unsigned my_seen = (unsigned)max(my_pos + 1 - my_lo, 0);
@@ -399,53 +404,45 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         const int lo_min = __builtin_amdgcn_readfirstlane(my_lo);
         const int lo_max = __builtin_amdgcn_readlane(my_lo, 31);
 
-        const int t_begin = blk.t_first + it0 * BN;
-        const int n_tiles = it1 - it0;
         const int last = blk.kend - 1;
-        const int32_t* table = SRC == kPaPacked ? nullptr : p.seqs.page_table + (int64_t)blk.seq * p.seqs.table_stride;
         const char* const kb0 = (const char*)p.k + (int64_t)blk.g * p.head_stride * EB;
         const char* const vb0 = (const char*)p.v + (int64_t)blk.g * p.head_stride * EB;
+        int page0 = 0;        // the page Ids[0] is of
+        bool some_bad = false;
 
         // Page ids of a tile: lane u < LD the page of this wave's rows of round u, lane 32 + j
         // that of keys 16 j .. 16 j + 15.
-        auto load_ids = [&](int t0) {
+        auto tile_ids = [&](int t0) __attribute__((always_inline)) {
             if constexpr (SRC == kPaPacked) return 0;
-            const int key = t0 + (lane < 32 ? wave * RPV + lane * RPU : (lane - 32) * 16);
-            return table[min(key, last) >> p.seqs.page_shift];
-        };
-        // Q8: the page of key t0 + tid
-        auto load_key_id = [&](int t0) {
-            if constexpr (!kQ8) return 0;
-            return table[min(t0 + tid, last) >> p.seqs.page_shift];
+            const int key = t0 + (lane < 32 ? wave * RPV + min(lane, LD - 1) * RPU : min(lane - 32, BN / 16 - 1) * 16);
+            return Ids[(min(key, last) >> shift) - page0];
         };
         // 16-key runs of the tile whose page is not there
-        auto bad_runs = [&](int ids) {
-            if constexpr (SRC == kPaPacked) return 0u;
-            return (unsigned)(__ballot((unsigned)ids >= (unsigned)p.seqs.n_pages) >> 32) & ((1u << (BN / 16)) - 1);
+        auto bad_runs = [&](int t0) __attribute__((always_inline)) {
+            if (SRC == kPaPacked || !some_bad) return 0u;
+            return (unsigned)(__ballot(tile_ids(t0) < 0) >> 32) & ((1u << (BN / 16)) - 1);
         };
-
-        // For round u of the tile at t0: the scalar byte offset of this wave's run of rows, and
-        // the rows the lane's offset is clamped to (rows past the last key repeat it: they are
+        // For round u of the tile at t0: the byte offset of this wave's run of rows (scalar), and
+        // how far the lane's row may go in it (rows past the last key repeat it: they are
         // masked, and must not be read).
         auto run_of = [&](int t0, int ids, int u, int& room) __attribute__((always_inline)) {
-            const int f = t0 + wave * RPV + u * RPU;
-            const int fc = min(f, last);
+            const int fc = min(t0 + wave * RPV + u * RPU, last);
             room = last - fc;
             if constexpr (SRC == kPaPacked) {
                 return (int64_t)(blk.beg + fc) * p.row_stride * EB;
             } else {
-                int id = __builtin_amdgcn_readlane(ids, u);
-                if ((unsigned)id >= (unsigned)p.seqs.n_pages) id = 0;
+                const int id = max(__builtin_amdgcn_readlane(ids, u), 0);
                 return ((int64_t)id * p.page_stride + (int64_t)(fc & ps1) * p.row_stride) * EB;
             }
         };
-        auto dma_tile = [&](int t0, int ids, uint16_t* kd, uint16_t* vd) __attribute__((always_inline)) {
+        auto dma_tile = [&](int t0, uint16_t* kd, uint16_t* vd) __attribute__((always_inline)) {
+            const int ids = tile_ids(t0);
             const bool full = t0 + BN - 1 <= last;
 #pragma unroll
             for (int u = 0; u < LD; u++) {
                 int room;
                 const int64_t at = run_of(t0, ids, u, room);
-                const int off = (full ? lrow : min(lrow, room)) * rsb + col[u];
+                const int off = (full ? lrow : min(lrow, room)) * rsb + col(u);
                 const int dst = (wave * 64 + u * NT) * 8;
                 pa_dma16(pa_rsrc(kb0 + at), kd + dst, off);
                 pa_dma16(pa_rsrc(vb0 + at), vd + dst, off);
@@ -453,21 +450,22 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         };
         uint4 kr[kQ8 ? LD : 1], vr[kQ8 ? LD : 1];
         float ks_r = 0.0f, vs_r = 1.0f;
-        auto load_q8 = [&](int t0, int ids, int key_id) __attribute__((always_inline)) {
+        auto load_q8 = [&](int t0) __attribute__((always_inline)) {
             if constexpr (kQ8) {
+                const int ids = tile_ids(t0);
                 const bool full = t0 + BN - 1 <= last;
 #pragma unroll
                 for (int u = 0; u < LD; u++) {
                     int room;
                     const int64_t at = run_of(t0, ids, u, room);
-                    const int off = (full ? lrow : min(lrow, room)) * rsb + col[u];
+                    const int off = (full ? lrow : min(lrow, room)) * rsb + col(u);
                     kr[u] = pa_load16(pa_rsrc(kb0 + at), off);
                     vr[u] = pa_load16(pa_rsrc(vb0 + at), off);
                 }
                 if (tid < BN) {
-                    const int id = (unsigned)key_id < (unsigned)p.seqs.n_pages ? key_id : 0;
-                    const int64_t at = (int64_t)id * p.scale_page_stride +
-                                       (int64_t)(min(t0 + tid, last) & ps1) * p.scale_row_stride +
+                    const int key = min(t0 + tid, last);
+                    const int id = max(Ids[(key >> shift) - page0], 0);
+                    const int64_t at = (int64_t)id * p.scale_page_stride + (int64_t)(key & ps1) * p.scale_row_stride +
                                        (int64_t)blk.g * p.scale_head_stride;
                     ks_r = p.k_scale[at];
                     vs_r = p.v_scale[at];
@@ -495,29 +493,17 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             }
         };
 
-        __syncthreads();  // the block before is done with every LDS buffer
-        int ids = 0, key_id = 0;
-        unsigned bad0 = 0, bad1 = 0;
-        if (n_tiles > 0) {
-            ids = load_ids(t_begin);
-            key_id = load_key_id(t_begin);
-            bad0 = bad_runs(ids);
-            if constexpr (kQ8) load_q8(t_begin, ids, key_id);
-            else dma_tile(t_begin, ids, Ks0, Vs0);
-            if (n_tiles > 1) {
-                ids = load_ids(t_begin + BN);
-                key_id = load_key_id(t_begin + BN);
-            }
-        }
-
         // ------------------------------------------------ Q: B operands, one row per lane column
         uint4 qf[D / 16];
         float q_mul = 1.0f;  // Q8: what the scores are multiplied by (bf16 rows are put in f16's range)
         {
+            const int h = blk.g * group + (min(wr0 + ln, n_pr - 1) - my_tok * group);
             const uint16_t* qr = (const uint16_t*)p.q + (int64_t)(blk.beg + my_tok) * p.q_row_stride +
-                                 (int64_t)my_h * p.q_head_stride;
+                                 (int64_t)h * p.q_head_stride;
 #pragma unroll
             for (int c = 0; c < D / 16; c++) qf[c] = *(const uint4*)(qr + 16 * c + 8 * lg);
+        }
+        auto prepare_q = [&]() __attribute__((always_inline)) {
             if constexpr (kQ8) {
                 if (p.dtype == GR_DTYPE_BF16) {
                     // bf16's 8 significant bits fit f16's 11: exact but for values 2^-24 below the row's largest
@@ -543,7 +529,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     }
                 }
             }
-        }
+        };
 
         pa_f32x16 o[D / 32];
 #pragma unroll
@@ -732,182 +718,261 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             }
         };
 
-        // Double-buffered tiles; ids are those of the tile after the one in flight.
-        if constexpr (kQ8) {
-            if (n_tiles > 0) store_q8(Ks0, Vs0, Sc0);
-            __syncthreads();
-            for (int it = 0; it < n_tiles; it += 2) {
-                const int t0 = t_begin + it * BN;
-                if (it + 1 < n_tiles) {
-                    bad1 = bad_runs(ids);
-                    load_q8(t0 + BN, ids, key_id);
-                    if (it + 2 < n_tiles) ids = load_ids(t0 + 2 * BN), key_id = load_key_id(t0 + 2 * BN);
+        // The tiles, run of page ids by run.
+        const int run_tiles = SRC == kPaPacked ? it1 - it0 : (int)(((int64_t)(kIds - 1) << shift) / BN);
+        for (int rt = it0; rt < it1; rt += run_tiles) {
+            const int t_begin = blk.t_first + rt * BN;
+            const int n_tiles = min(it1 - rt, run_tiles);
+            __syncthreads();  // what ran before is done with every LDS array
+            if constexpr (SRC != kPaPacked) {
+                const int32_t* table = p.seqs.page_table + (int64_t)blk.seq * p.seqs.table_stride;
+                page0 = t_begin >> shift;
+                const int n_ids = (min(last, t_begin + n_tiles * BN - 1) >> shift) - page0 + 1;
+                int bad = 0;
+                for (int i = tid; i < n_ids; i += NT) {
+                    const int id = table[page0 + i];
+                    const bool there = (unsigned)id < (unsigned)p.seqs.n_pages;
+                    Ids[i] = there ? id : -1;
+                    bad |= !there;
                 }
-                compute_tile(Ks0, Vs0, Sc0, t0, bad0);
-                if (it + 1 >= n_tiles) break;
-                store_q8(Ks1, Vs1, Sc1);
-                __syncthreads();
-                if (it + 2 < n_tiles) {
-                    bad0 = bad_runs(ids);
-                    load_q8(t0 + 2 * BN, ids, key_id);
-                    if (it + 3 < n_tiles) ids = load_ids(t0 + 3 * BN), key_id = load_key_id(t0 + 3 * BN);
-                }
-                compute_tile(Ks1, Vs1, Sc1, t0 + BN, bad1);
-                if (it + 2 < n_tiles) store_q8(Ks0, Vs0, Sc0);
-                __syncthreads();
+                some_bad = __syncthreads_or(bad);
             }
-        } else {
-            for (int it = 0; it < n_tiles; it += 2) {
-                const int t0 = t_begin + it * BN;
-                pa_wait_vmem();   // this thread's part of tile it is in LDS
-                __syncthreads();  // ... everyone's, and tile it - 1's buffers are free
-                if (it + 1 < n_tiles) {
-                    bad1 = bad_runs(ids);
-                    dma_tile(t0 + BN, ids, Ks1, Vs1);
-                    if (it + 2 < n_tiles) ids = load_ids(t0 + 2 * BN);
-                }
-                compute_tile(Ks0, Vs0, Sc0, t0, bad0);
-                if (it + 1 >= n_tiles) break;
-                pa_wait_vmem();
+            if constexpr (kQ8) {
+                load_q8(t_begin);
+                if (rt == it0) prepare_q();
+                store_q8(Ks0, Vs0, Sc0);
                 __syncthreads();
-                if (it + 2 < n_tiles) {
-                    bad0 = bad_runs(ids);
-                    dma_tile(t0 + 2 * BN, ids, Ks0, Vs0);
-                    if (it + 3 < n_tiles) ids = load_ids(t0 + 3 * BN);
+                for (int it = 0; it < n_tiles; it += 2) {
+                    const int t0 = t_begin + it * BN;
+                    if (it + 1 < n_tiles) load_q8(t0 + BN);
+                    compute_tile(Ks0, Vs0, Sc0, t0, bad_runs(t0));
+                    if (it + 1 >= n_tiles) break;
+                    store_q8(Ks1, Vs1, Sc1);
+                    __syncthreads();
+                    if (it + 2 < n_tiles) load_q8(t0 + 2 * BN);
+                    compute_tile(Ks1, Vs1, Sc1, t0 + BN, bad_runs(t0 + BN));
+                    if (it + 2 < n_tiles) store_q8(Ks0, Vs0, Sc0);
+                    __syncthreads();
                 }
-                compute_tile(Ks1, Vs1, Sc1, t0 + BN, bad1);
+            } else {
+                auto kbuf = [&](auto i) __attribute__((always_inline)) -> uint16_t* {
+                    constexpr int I = decltype(i)::value % NBUF;
+                    if constexpr (I == 0) return Ks0;
+                    else if constexpr (I == 1) return Ks1;
+                    else if constexpr (I == 2) return Ks2;
+                    else return Ks3;
+                };
+                auto vbuf = [&](auto i) __attribute__((always_inline)) -> uint16_t* {
+                    constexpr int I = decltype(i)::value % NBUF;
+                    if constexpr (I == 0) return Vs0;
+                    else if constexpr (I == 1) return Vs1;
+                    else if constexpr (I == 2) return Vs2;
+                    else return Vs3;
+                };
+                // tile it (buffer I): wait until it is in LDS, send for the tile NBUF - 1 later, compute
+                auto step = [&](auto i, int it) __attribute__((always_inline)) {
+                    constexpr int I = decltype(i)::value;
+                    const int t0 = t_begin + it * BN;
+                    if (it + NBUF - 2 < n_tiles) pa_wait_vmem<(NBUF - 2) * 2 * LD>();
+                    else pa_wait_vmem<0>();
+                    __syncthreads();  // everyone's part of it is, and tile it - 1's buffer is free
+                    if (it + NBUF - 1 < n_tiles)
+                        dma_tile(t0 + (NBUF - 1) * BN, kbuf(std::integral_constant<int, I + NBUF - 1>{}),
+                                 vbuf(std::integral_constant<int, I + NBUF - 1>{}));
+                    compute_tile(kbuf(i), vbuf(i), Sc0, t0, bad_runs(t0));
+                };
+                using std::integral_constant;
+                dma_tile(t_begin, Ks0, Vs0);
+                if constexpr (NBUF == 4) {
+                    if (n_tiles > 1) dma_tile(t_begin + BN, Ks1, Vs1);
+                    if (n_tiles > 2) dma_tile(t_begin + 2 * BN, Ks2, Vs2);
+                }
+                for (int it = 0; it < n_tiles; it += NBUF) {
+                    step(integral_constant<int, 0>{}, it);
+                    if (it + 1 >= n_tiles) break;
+                    step(integral_constant<int, 1>{}, it + 1);
+                    if constexpr (NBUF == 4) {
+                        if (it + 2 >= n_tiles) break;
+                        step(integral_constant<int, 2>{}, it + 2);
+                        if (it + 3 >= n_tiles) break;
+                        step(integral_constant<int, 3>{}, it + 3);
+                    }
+                }
             }
         }
 
         // ------------------------------------------------ key parts join, then out
         float lsum = pa_xsum32(lrow_sum);
+        // the rows again (not kept through the loop)
+        int ln2 = ln;
+        asm volatile("" : "+v"(ln2));
+        const int row = wr0 + ln2;
+        const bool row_ok = row < n_pr;
+        const int tok = token_of(row);
         if constexpr (KH > 1) {
-            // key parts 1 .. hand (O, m, l) of their rows to part 0, one part after another,
-            // through the tile buffers: O = O0 2^(m0 - m) + O1 2^(m1 - m), m = max(m0, m1)
+            // Every key part leaves (O, m, l) of its rows in the tile buffers; part k then adds up the
+            // D / 32 / KH (at least one) O^T tiles that are its share: O = sum O_k 2^(m_k - m), m = max m_k.
             constexpr int NO = D / 32 * 16;
-            static_assert(RW * NO * 64 * 4 <= 2 * BN * D * 2 && RW * 2 * 64 * 4 <= BN * D * 2, "merge buffers");
-#pragma unroll 1
-            for (int part = 1; part < KH; part++) {
-                __syncthreads();
-                float* const half0 = (float*)Ks0;
-                float* const half1 = (float*)Ks1;
-                float* const ml = (float*)Vs0 + rw * 128;
-                constexpr int NH = BN * D * 2 / 4;  // floats per buffer
-                auto at = [&](int i) -> float& {
-                    const int x = (rw * NO + i) * 64 + lane;
-                    return x < NH ? half0[x] : half1[x - NH];
-                };
-                if (kh == part) {
+            static_assert(RW == 1 && KH * NO * 64 * 4 <= 2 * BN * D * 2 && KH * 128 * 4 <= BN * D * 2, "merge buffers");
+            constexpr int NH = BN * D * 2 / 4;  // floats per buffer
+            static_assert(NH % (NO * 64) == 0, "a part's O lies in one buffer");
+            auto part_o = [&](int k) { return (k * NO * 64 < NH ? (float*)Ks0 : (float*)Ks1) + k * NO * 64 % NH; };
+            float* const ml = (float*)Vs0;
+            __syncthreads();
+            float* const mine = part_o(kh);
 #pragma unroll
-                    for (int dt = 0; dt < D / 32; dt++)
+            for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
-                        for (int e = 0; e < 16; e++) at(dt * 16 + e) = o[dt][e];
-                    ml[lane] = mrow;
-                    ml[64 + lane] = lsum;
+                for (int j = 0; j < 4; j++)
+                    *(float4*)(mine + ((4 * dt + j) * 64 + lane) * 4) =
+                        make_float4(o[dt][4 * j + 0], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
+            ml[kh * 128 + lane] = mrow;
+            ml[kh * 128 + 64 + lane] = lsum;
+            __syncthreads();
+            float mk[KH];
+            mrow = kPaNone;
+#pragma unroll
+            for (int k = 0; k < KH; k++) mk[k] = ml[k * 128 + lane], mrow = fmaxf(mrow, mk[k]);
+            lsum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KH; k++) {
+                mk[k] = __builtin_amdgcn_exp2f(mk[k] - mrow);
+                lsum = fmaf(ml[k * 128 + 64 + lane], mk[k], lsum);
+            }
+            constexpr int SH = D / 8 / KH;  // float4s of a part's share
+#pragma unroll
+            for (int i = 0; i < SH; i++) {
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < KH; k++) {
+                    const float4 y = *(const float4*)(part_o(k) + ((kh * SH + i) * 64 + lane) * 4);
+                    x.x = fmaf(y.x, mk[k], x.x), x.y = fmaf(y.y, mk[k], x.y);
+                    x.z = fmaf(y.z, mk[k], x.z), x.w = fmaf(y.w, mk[k], x.w);
                 }
-                __syncthreads();
-                if (kh == 0) {
-                    const float m1 = ml[lane], l1 = ml[64 + lane];
-                    const float mm = fmaxf(mrow, m1);
-                    const float a0 = __builtin_amdgcn_exp2f(mrow - mm), a1 = __builtin_amdgcn_exp2f(m1 - mm);
-                    mrow = mm;
-                    lsum = lsum * a0 + l1 * a1;
-#pragma unroll
-                    for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) o[dt][e] = o[dt][e] * a0 + at(dt * 16 + e) * a1;
-                }
+                o[i / 4][i % 4 * 4 + 0] = x.x, o[i / 4][i % 4 * 4 + 1] = x.y;
+                o[i / 4][i % 4 * 4 + 2] = x.z, o[i / 4][i % 4 * 4 + 3] = x.w;
             }
         }
-        if (kh != 0 || !wave_active) continue;
+        if (!wave_active || !row_ok) continue;
+        constexpr int N4 = D / 8 / KH;         // float4s of the row that this lane has ...
+        const int first4 = KH > 1 ? kh * N4 : 0;  // ... from this one on
         if constexpr (STREAM) {
             if (!whole) {
                 float* const ws = (float*)p.workspace + (int64_t)(slot * RW + rw) * (32 * D + 64);
-                if (row_ok) {
 #pragma unroll
-                    for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-                        for (int jb = 0; jb < 4; jb++)
-                            *(float4*)(ws + ((4 * dt + jb) * 64 + lane) * 4) =
-                                make_float4(o[dt][4 * jb + 0], o[dt][4 * jb + 1], o[dt][4 * jb + 2], o[dt][4 * jb + 3]);
-                    if (lg == 0) {
-                        ws[32 * D + ln] = mrow;
-                        ws[32 * D + 32 + ln] = lsum;
-                    }
+                for (int i = 0; i < N4; i++)
+                    *(float4*)(ws + ((first4 + i) * 64 + lane) * 4) =
+                        make_float4(o[i / 4][i % 4 * 4 + 0], o[i / 4][i % 4 * 4 + 1], o[i / 4][i % 4 * 4 + 2],
+                                    o[i / 4][i % 4 * 4 + 3]);
+                if (lg == 0 && kh == 0) {
+                    ws[32 * D + ln] = mrow;
+                    ws[32 * D + 32 + ln] = lsum;
                 }
                 continue;
             }
         }
-        if (row_ok) {
-            const float inv = lsum != 0.0f ? 1.0f / lsum : 0.0f;
-            uint16_t* orow = (uint16_t*)p.out + (int64_t)(blk.beg + my_tok) * p.out_row_stride +
-                             (int64_t)my_h * p.out_head_stride;
-            const bool f16 = p.dtype == GR_DTYPE_F16;
+        const float inv = lsum != 0.0f ? 1.0f / lsum : 0.0f;
+        uint16_t* orow = (uint16_t*)p.out + (int64_t)(blk.beg + tok) * p.out_row_stride +
+                         (int64_t)(blk.g * group + (row - tok * group)) * p.out_head_stride;
+        const bool f16 = kQ8 ? p.dtype == GR_DTYPE_F16 : std::is_same_v<DT, F16>;
 #pragma unroll
-            for (int dt = 0; dt < D / 32; dt++)
+        for (int i = 0; i < N4; i++) {
+            float x[4];
 #pragma unroll
-                for (int jb = 0; jb < 4; jb++) {
-                    float x[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = o[dt][4 * jb + e] * inv;
-                    uint2 r;
-                    if (kQ8 ? f16 : std::is_same_v<DT, F16>)
-                        r = make_uint2(PaMat<F16>::pack2(x[0], x[1]), PaMat<F16>::pack2(x[2], x[3]));
-                    else
-                        r = make_uint2(PaMat<BF16>::pack2(x[0], x[1]), PaMat<BF16>::pack2(x[2], x[3]));
-                    *(uint2*)(orow + 32 * dt + 8 * jb + 4 * lg) = r;
-                }
+            for (int e = 0; e < 4; e++) x[e] = o[i / 4][i % 4 * 4 + e] * inv;
+            uint2 r;
+            if (f16) r = make_uint2(PaMat<F16>::pack2(x[0], x[1]), PaMat<F16>::pack2(x[2], x[3]));
+            else r = make_uint2(PaMat<BF16>::pack2(x[0], x[1]), PaMat<BF16>::pack2(x[2], x[3]));
+            *(uint2*)(orow + 8 * (first4 + i) + 4 * lg) = r;
         }
     }
 }
 
 // Joins the pieces of the block that boundary w (the start of range w) is the first to cut;
-// blockIdx.y: a row group of it.
+// blockIdx.y: a row group of it.  Thread (row, 4 elements) runs over the pieces; with few rows
+// the workgroup's spare threads share a row's pieces among them and add up in LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunch p, const int n_ranges) {
     constexpr int D = T::D, RW = T::RW, BM = T::BM, BN = T::BN;
-    const int64_t total = pa_stream_total<BM, BN>(p);
-    const int64_t q = pa_stream_q(total, n_ranges);
+    constexpr int kUnit = 32 * D + 64;
+    __shared__ __attribute__((aligned(16))) float4 So[256];
+    __shared__ float Sl[256];
+    __shared__ float Sm[256];
+    const PaSeq c0 = pa_seq<BM, BN>(p, threadIdx.x & 63);
+    const int total = pa_stream_total<BM, BN>(p, c0);
+    const int q = pa_stream_q(total, n_ranges, p.least);
     const int w0 = (int)blockIdx.x;  // the range before the boundary
-    const int64_t x = (w0 + 1) * q;
-    if (x >= total) return;
-    const PaPlace pl = pa_stream_find<BM, BN>(p, x);
-    if (pl.at == 0 || pl.at > q) return;  // no cut here, or an earlier boundary was in this block
+    if ((int64_t)(w0 + 1) * q >= total) return;
     PaBlock blk;
-    blk.seq = pl.seq, blk.rb = pl.rb, blk.g = pl.g;
-    pa_block<BM, BN>(p, blk);
+    const int at = pa_stream_find<BM, BN>(p, c0, (w0 + 1) * q, blk);
+    if (at == 0 || at > q) return;  // no cut here, or an earlier boundary was in this block
     const int group = p.n_heads / p.n_kv_heads;
     const int r0 = blk.rb * BM + (int)blockIdx.y * 32;
     const int nr = min(32, blk.n * group - r0);
     if (nr <= 0) return;
-    const int64_t start = x - pl.at;                 // the block's first place
-    const int n_pieces = (int)((start + pl.vt - 1) / q) - w0 + 1;
-    constexpr int kUnit = 32 * D + 64;
-    const float* const ws = (const float*)p.workspace;
-    // piece i: range w0 + i; its slot and whether it has tiles
-    auto piece = [&](int i) -> const float* {
-        const int w = w0 + i;
-        const int64_t a = max((int64_t)w * q, start) - start, b = min((int64_t)(w + 1) * q, start + pl.vt) - start;
-        if (pa_real(a, blk.n_tiles, pl.vt) == pa_real(b, blk.n_tiles, pl.vt)) return nullptr;
-        return ws + ((int64_t)(2 * w + (a == 0 ? 1 : 0)) * RW + (int)blockIdx.y) * kUnit;
-    };
-    for (int i = threadIdx.x; i < nr * (D / 4); i += 256) {
-        const int r = i % nr, c = i / nr;            // row, float4 c of it: (c >> 1)-th group of 8, lane half c & 1
-        float m = kPaNone;
-        for (int k = 0; k < n_pieces; k++) {
-            const float* u = piece(k);
-            if (u) m = fmaxf(m, u[32 * D + r]);
-        }
-        float l = 0.0f;
+    // piece k is range w0 + k's: tiles [k q - (q - at), (k + 1) q - (q - at)) of the block, those in
+    // [0, n_tiles); the first one started inside its range (slot 1 of it), the others at its start
+    const int lead = q - at;
+    const int n_pieces = blk.n_tiles > 0 ? (blk.n_tiles + lead - 1) / q + 1 : 0;
+    const float* const ws = (const float*)p.workspace + (int64_t)blockIdx.y * kUnit;
+    auto piece = [&](int k) { return ws + (int64_t)(2 * (w0 + k) + (k == 0 ? 1 : 0)) * RW * kUnit; };
+    const int tid = threadIdx.x;
+    const int n_items = nr * (D / 4);
+    int parts = 1;  // threads per item, a power of two
+    while (n_items * parts * 2 <= 256 && parts * 2 <= n_pieces) parts *= 2;
+    const int per = 256 / parts;  // items at once
+    const int my_part = tid / per;
+    for (int i0 = 0; i0 < n_items; i0 += per) {
+        const int i = i0 + tid % per;
+        const bool mine = i < n_items;
+        const int r = mine ? i % nr : 0, c = mine ? i / nr : 0;  // row; float4 c: 8-group c / 2, half c & 1
+        const int e = ((c >> 1) * 64 + (c & 1) * 32 + r) * 4;
+        float m = kPaNone, l = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < n_pieces; k++) {
-            const float* u = piece(k);
-            if (!u) continue;
-            const float a = __builtin_amdgcn_exp2f(u[32 * D + r] - m);
-            const float4 v = *(const float4*)(u + ((c >> 1) * 64 + (c & 1) * 32 + r) * 4);
-            l = fmaf(u[32 * D + 32 + r], a, l);
-            o.x = fmaf(v.x, a, o.x), o.y = fmaf(v.y, a, o.y), o.z = fmaf(v.z, a, o.z), o.w = fmaf(v.w, a, o.w);
+        if (mine) {
+            constexpr int U = 4;  // pieces at once
+            for (int k0 = my_part; k0 < n_pieces; k0 += U * parts) {
+                float4 v[U];
+                float mk[U], lk[U];
+                float top = m;
+#pragma unroll
+                for (int j = 0; j < U; j++) {
+                    const float* u = piece(min(k0 + j * parts, n_pieces - 1));
+                    v[j] = *(const float4*)(u + e);
+                    mk[j] = k0 + j * parts < n_pieces ? u[32 * D + r] : -INFINITY;
+                    lk[j] = u[32 * D + 32 + r];
+                    top = fmaxf(top, mk[j]);
+                }
+                const float a = __builtin_amdgcn_exp2f(m - top);
+                m = top;
+                l *= a, o.x *= a, o.y *= a, o.z *= a, o.w *= a;
+#pragma unroll
+                for (int j = 0; j < U; j++) {
+                    const float b = __builtin_amdgcn_exp2f(mk[j] - top);
+                    if (k0 + j * parts < n_pieces) {
+                        l = fmaf(lk[j], b, l);
+                        o.x = fmaf(v[j].x, b, o.x), o.y = fmaf(v[j].y, b, o.y);
+                        o.z = fmaf(v[j].z, b, o.z), o.w = fmaf(v[j].w, b, o.w);
+                    }
+                }
+            }
         }
+        if (parts > 1) {  // n_items * parts <= 256: one round
+            So[tid] = o, Sl[tid] = l, Sm[tid] = m;
+            __syncthreads();
+            if (my_part != 0 || !mine) return;
+            float top = m;
+            for (int k = 1; k < parts; k++) top = fmaxf(top, Sm[tid + k * per]);
+            float a = __builtin_amdgcn_exp2f(m - top);
+            l *= a, o.x *= a, o.y *= a, o.z *= a, o.w *= a;
+            for (int k = 1; k < parts; k++) {
+                const float4 v = So[tid + k * per];
+                a = __builtin_amdgcn_exp2f(Sm[tid + k * per] - top);
+                l = fmaf(Sl[tid + k * per], a, l);
+                o.x = fmaf(v.x, a, o.x), o.y = fmaf(v.y, a, o.y), o.z = fmaf(v.z, a, o.z), o.w = fmaf(v.w, a, o.w);
+            }
+        }
+        if (!mine) continue;
         const float inv = l != 0.0f ? 1.0f / l : 0.0f;
         const int tok = (r0 + r) / group, h = blk.g * group + (r0 + r) % group;
         uint16_t* out = (uint16_t*)p.out + (int64_t)(blk.beg + tok) * p.out_row_stride + (int64_t)h * p.out_head_stride + 4 * c;
@@ -922,11 +987,16 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunc
 
 // ---------------------------------------------------------------- launches
 
-// Blocks of a launch at most: every sequence's last block may be partly filled.
+// Blocks of a KV head in a launch at most: every sequence's last block may be partly filled.
 template <typename T>
 int64_t pa_max_blocks(const PagedAttnLaunch& p) {
     const int64_t rows = (int64_t)p.seqs.n_rows * (p.n_heads / p.n_kv_heads);
-    return (rows / T::BM + std::min<int64_t>(p.seqs.n_seq, p.seqs.n_rows)) * p.n_kv_heads;
+    return rows / T::BM + std::min<int64_t>(p.seqs.n_seq, p.seqs.n_rows);
+}
+// Places of the stream at most.
+template <typename T>
+int64_t pa_max_places(const PagedAttnLaunch& p) {
+    return pa_max_blocks<T>(p) * p.n_kv_heads * (p.seqs.max_len / T::BN + 1);
 }
 
 template <typename T>
@@ -935,13 +1005,14 @@ size_t pa_ws_bytes(int ranges) { return (size_t)2 * ranges * T::RW * (32 * T::D 
 template <typename DT, typename T, int SRC>
 hipError_t pa_launch_ordered(const PagedAttnLaunch& p, hipStream_t st) {
     // whole rounds of the XCDs for every KV head
-    const int64_t per = (pa_max_blocks<T>(p) / p.n_kv_heads + 7) / 8 * 8;
+    const int64_t per = (pa_max_blocks<T>(p) + 7) / 8 * 8;
     paged_attn_kernel<DT, T, SRC, false><<<dim3((unsigned)(per * p.n_kv_heads)), T::NT, 0, st>>>(p);
     return hipGetLastError();
 }
 
 template <typename DT, typename T, int SRC>
-hipError_t pa_launch_stream(const PagedAttnLaunch& p, int ranges, hipStream_t st) {
+hipError_t pa_launch_stream(PagedAttnLaunch p, int ranges, int least, hipStream_t st) {
+    p.least = least;
     paged_attn_kernel<DT, T, SRC, true><<<dim3((unsigned)ranges), T::NT, 0, st>>>(p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -949,7 +1020,9 @@ hipError_t pa_launch_stream(const PagedAttnLaunch& p, int ranges, hipStream_t st
     return hipGetLastError();
 }
 
-// One (element type, source) of a head_dim: the tiles it is built for and which it takes.
+bool paged_attn_fits_d64(const PagedAttnLaunch& p);
+bool paged_attn_fits_d128(const PagedAttnLaunch& p);
+bool paged_attn_fits_d256(const PagedAttnLaunch& p);
 size_t paged_attn_ws_d64(const PagedAttnLaunch& p);
 size_t paged_attn_ws_d128(const PagedAttnLaunch& p);
 size_t paged_attn_ws_d256(const PagedAttnLaunch& p);
@@ -957,13 +1030,14 @@ hipError_t launch_paged_attn_d64(const PagedAttnLaunch& p, hipStream_t st);
 hipError_t launch_paged_attn_d128(const PagedAttnLaunch& p, hipStream_t st);
 hipError_t launch_paged_attn_d256(const PagedAttnLaunch& p, hipStream_t st);
 
-// Few: blocks of few rows, key parts; Mid, Big: whole row blocks.
-template <typename Few, typename Mid, typename Big>
+// The kernels of a head_dim and which of them a call takes.  Few: blocks of few rows, key
+// parts (FewQ8 over Q8 pages); Mid, Big: whole row blocks.
+template <typename Few, typename FewQ8, typename Mid, typename Big>
 struct PaKernels {
     enum Kind { kFew, kMidStream, kMid, kBig };
     static constexpr int kCus = 256;
-    static constexpr int few_ranges = kCus * std::max(1, Few::OCC * 4 / Few::NW);
-    static constexpr int mid_ranges = kCus * std::max(1, Mid::OCC * 4 / Mid::NW);
+    template <typename T>
+    static constexpr int ranges = kCus * std::max(1, T::OCC * 4 / T::NW);
 
     static Kind kind(const PagedAttnLaunch& p) {
         const int64_t group = p.n_heads / p.n_kv_heads;
@@ -975,16 +1049,20 @@ struct PaKernels {
     }
     static size_t ws(const PagedAttnLaunch& p) {
         switch (kind(p)) {
-            case kFew: return pa_ws_bytes<Few>(few_ranges);
-            case kMidStream: return pa_ws_bytes<Mid>(mid_ranges);
+            case kFew: return p.kv_dtype == GR_DTYPE_Q8 ? pa_ws_bytes<FewQ8>(ranges<FewQ8>) : pa_ws_bytes<Few>(ranges<Few>);
+            case kMidStream: return pa_ws_bytes<Mid>(ranges<Mid>);
             default: return 256;
         }
     }
+    static bool fits(const PagedAttnLaunch& p) {
+        return std::max({pa_max_places<Few>(p), pa_max_places<FewQ8>(p), pa_max_places<Mid>(p)}) < INT32_MAX;
+    }
     template <typename DT, int SRC>
     static hipError_t launch(const PagedAttnLaunch& p, hipStream_t st) {
+        using F = std::conditional_t<SRC == kPaPagesQ8, FewQ8, Few>;
         switch (kind(p)) {
-            case kFew: return pa_launch_stream<DT, Few, SRC>(p, few_ranges, st);
-            case kMidStream: return pa_launch_stream<DT, Mid, SRC>(p, mid_ranges, st);
+            case kFew: return pa_launch_stream<DT, F, SRC>(p, ranges<F>, 1, st);
+            case kMidStream: return pa_launch_stream<DT, Mid, SRC>(p, ranges<Mid>, 1, st);
             case kMid: return pa_launch_ordered<DT, Mid, SRC>(p, st);
             default: return pa_launch_ordered<DT, Big, SRC>(p, st);
         }

@@ -5,8 +5,9 @@
 
 namespace gr {
 
-using K256 = PaKernels<PaTile<256, 1, 2, 64, 1>, PaTile<256, 4, 1, 64, 1>, PaTile<256, 4, 1, 64, 1>>;
+using K256 = PaKernels<PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 4, 1, 64, 2, 1>, PaTile<256, 4, 1, 64, 2, 1>>;
 
+bool paged_attn_fits_d256(const PagedAttnLaunch& p) { return K256::fits(p); }
 size_t paged_attn_ws_d256(const PagedAttnLaunch& p) { return K256::ws(p); }
 hipError_t launch_paged_attn_d256(const PagedAttnLaunch& p, hipStream_t st) { return K256::launch_any(p, st); }
 

@@ -294,14 +294,19 @@ class _DeviceCall:
     device: torch.device
 
     def _enqueue(self, stream, fn, *args) -> None:
+        index = self.device.index
         if stream is None:
-            stream = torch.cuda.current_stream(self.device)
-        _need(stream.device == self.device, f"the call's tensors live on {self.device}, the stream on {stream.device}")
-        if torch.cuda.current_device() == self.device.index:
-            ffi.check(fn(*args, stream.cuda_stream))
+            raw = torch._C._cuda_getCurrentRawStream(index)
         else:
-            with torch.cuda.device(self.device):
-                ffi.check(fn(*args, stream.cuda_stream))
+            _need(stream.device == self.device, f"the call's tensors live on {self.device}, the stream on {stream.device}")
+            raw = stream.cuda_stream
+        if torch._C._cuda_getDevice() == index:
+            rc = fn(*args, raw)
+        else:
+            with torch.cuda.device(index):
+                rc = fn(*args, raw)
+        if rc:
+            ffi.check(rc)
 
 
 class PagedCache:

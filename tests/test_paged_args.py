@@ -147,6 +147,14 @@ def test_bad_packed_args(pkg, kw, msg):
     assert L.gr_packed_attention_workspace_size(packed(ffi, **kw)) == 0
 
 
+def test_more_work_than_can_be_numbered(pkg):
+    from gguf_runner_amd import ffi
+    L = ffi.lib()
+    big = dict(n_seq=1 << 20, n_rows=1 << 20, table_pages=1 << 20, table_stride=1 << 20)
+    refused(ffi, L.gr_paged_attention(cache(ffi), batch(ffi, **big), attn(ffi), None), "divide the batch")
+    assert L.gr_paged_attention_workspace_size(cache(ffi), batch(ffi, **big), attn(ffi)) == 0
+
+
 def test_null_and_workspace(pkg):
     from gguf_runner_amd import ffi
     L, c, b, a = ffi.lib(), cache(ffi), batch(ffi), attn(ffi)
