@@ -82,6 +82,9 @@ struct PaTile {
     static constexpr int D = D_, RW = RW_, KH = KH_, BN = BN_, NBUF = NBUF_, OCC = OCC_;
     static constexpr int NW = RW * KH, NT = NW * 64, BM = RW * 32;
     static_assert(BN % (32 * KH) == 0, "every key part has its sub-tiles");
+    static constexpr int kLds = 4 * NBUF * BN * D + 4096 + 24 * BN;  // at most (page ids, Q8 scales)
+    // workgroups a CU holds: by waves, and by its 160 KB of LDS
+    static constexpr int kPerCu = OCC * 4 / NW < 163840 / kLds ? (OCC * 4 / NW < 1 ? 1 : OCC * 4 / NW) : 163840 / kLds;
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t pa_rsrc(const void* base) {
@@ -138,6 +141,17 @@ __device__ __forceinline__ uint4 pa_cvt8(uint32_t x, uint32_t y) {
 constexpr float kPaNone = -1e30f;     // m of a row that has seen no key
 constexpr float kPaLazy = 8.0f;       // m is only raised for tile maxima this far above it: p <= 2^8
 constexpr float kPaLeastScale = 7.8886091e-31f;  // 2^-100: smaller v_scales count as this in m and l
+
+// The magnitudes of two 16-bit floats; the finite ones of eight (others 0).
+__device__ __forceinline__ pa_u16x2 pa_mag(uint32_t x) { return __builtin_bit_cast(pa_u16x2, x & 0x7fff7fffu); }
+template <typename M>
+__device__ __forceinline__ uint4 pa_finite(const uint4& a) {
+    auto two = [](uint32_t x) {
+        const uint32_t lo = (x & 0x7fffu) < M::kInf ? 0xffffu : 0u, hi = (x >> 16 & 0x7fffu) < M::kInf ? 0xffff0000u : 0u;
+        return x & (lo | hi);
+    };
+    return make_uint4(two(a.x), two(a.y), two(a.z), two(a.w));
+}
 
 // ---------------------------------------------------------------- schedules
 
@@ -336,13 +350,20 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     const int swz_k = pa_swz<D>(ln & 15);
     const int gi = lane & 15;
     const int v_chunk = 2 * ((lane >> 4) & 1) + ((gi & 3) >> 1);
-    int v_base[2], v_swz[2];
+    // V^T fragments (ds_read_b64_tr_b16): lane i of a 16-lane group supplies row i / 4, columns
+    // 4 (i % 4) .. +3 of a 4 x 16 block and receives its column i.  v_off: the byte offset of
+    // O^T tile dt's block b, less where the V arrays start in LDS, which keeps every other
+    // part of the address within the instruction's 16-bit offset.
+    constexpr int kVAt = NBUF * BN * D * 2;
+    int v_off[D / 32][2];
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
-        const int r = 8 * b + 4 * lg + (gi >> 2);
-        v_base[b] = r * D + (gi & 1) * 4;
-        v_swz[b] = pa_swz<D>(r & 15);
-    }
+    for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int r = 8 * b + 4 * lg + (gi >> 2);
+            v_off[dt][b] = kVAt + 2 * (r * D + (gi & 1) * 4 + (((4 * dt + v_chunk) ^ pa_swz<D>(r & 15)) << 3));
+            asm volatile("" : "+v"(v_off[dt][b]));
+        }
 
     // ------------------------------------------------ the workgroup's range
     const PaSeq c0 = pa_seq<BM, BN>(p, lane);
@@ -408,7 +429,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         const char* const kb0 = (const char*)p.k + (int64_t)blk.g * p.head_stride * EB;
         const char* const vb0 = (const char*)p.v + (int64_t)blk.g * p.head_stride * EB;
         int page0 = 0;        // the page Ids[0] is of
-        bool some_bad = false;
+        bool some_bad = false, ever_bad = false;  // in the run, in a run so far
 
         // Page ids of a tile: lane u < LD the page of this wave's rows of round u, lane 32 + j
         // that of keys 16 j .. 16 j + 15.
@@ -503,6 +524,13 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
 #pragma unroll
             for (int c = 0; c < D / 16; c++) qf[c] = *(const uint4*)(qr + 16 * c + 8 * lg);
         }
+        // Q is in its registers from here on: without a use in front of the tile loop its first
+        // product would wait for every load in flight, the next tile's among them.
+        auto settle_q = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < D / 16; c++)
+                asm volatile("" : "+v"(qf[c].x), "+v"(qf[c].y), "+v"(qf[c].z), "+v"(qf[c].w));
+        };
         auto prepare_q = [&]() __attribute__((always_inline)) {
             if constexpr (kQ8) {
                 if (p.dtype == GR_DTYPE_BF16) {
@@ -537,11 +565,15 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
 #pragma unroll
             for (int e = 0; e < 16; e++) o[dt][e] = 0.0f;
         float mrow = kPaNone, lrow_sum = 0.0f;
+        bool odd = false;  // some partly hidden sub-tile has V elements that are not finite
         const float c2 = p.scale_log2;
 
-        // One 32-key sub-tile: keys ts .. ts + 31, rows 32 sb .. of the tile; bad: its two
-        // 16-key runs that are not there.
-        auto subtile = [&](const uint16_t* kb, const uint16_t* vb, const float* sc, int sb, int ts, unsigned bad) __attribute__((always_inline)) {
+        // One 32-key sub-tile: keys ts .. ts + 31, rows 32 sb .. of the tile; masked: some row of
+        // the wave does not see all of them (bad: its two 16-key runs that are not there).
+        auto subtile = [&](auto masked, const uint16_t* kb, const uint16_t* vb, const float* sc, int sb, int ts,
+                           unsigned bad) __attribute__((always_inline)) {
+            constexpr bool kMasked = decltype(masked)::value;
+            __builtin_amdgcn_sched_barrier(0);  // sub-tiles are not interleaved: the registers hold one
             const pa_f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             __builtin_amdgcn_s_setprio(1);
             pa_f32x16 s;
@@ -555,8 +587,8 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                 pa_i16x4 part[2];
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
-                    const int off = (32 * sb + 16 * t) * D + v_base[b] + (((4 * dt + v_chunk) ^ v_swz[b]) << 3);
-                    part[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GR_PA_LDS pa_i16x4*)(vb + off));
+                    const char* at = (const char*)vb - kVAt + (32 * sb + 16 * t) * D * 2 + v_off[dt][b];
+                    part[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GR_PA_LDS pa_i16x4*)at);
                 }
                 const uint2 lo = __builtin_bit_cast(uint2, part[0]);
                 const uint2 hi = __builtin_bit_cast(uint2, part[1]);
@@ -584,18 +616,13 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     s[4 * j + 3] = fmaf(s[4 * j + 3] * q_mul, a.w, b.w);
                 }
             }
-            const bool need_mask = ts + 31 > hi_min || ts < lo_max || bad;
-            unsigned seen = 0xffffu;  // bit e: the lane's row sees the key of element e
-            if (need_mask) {
-                const int kb0_ = ts + 4 * lg - my_lo;
-                seen = 0;
+            if constexpr (kMasked) {
+                const int k0 = ts + 4 * lg - my_lo;
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    seen |= ((unsigned)(kb0_ + 8 * (e >> 2) + (e & 3)) < my_seen ? 1u : 0u) << e;
-                if (bad & 1) seen &= 0xff00u;
-                if (bad & 2) seen &= 0x00ffu;
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[e] = seen >> e & 1 ? s[e] : -INFINITY;
+                for (int e = 0; e < 16; e++) {
+                    const bool seen = (unsigned)(k0 + 8 * (e >> 2) + (e & 3)) < my_seen && !(bad >> (e >> 3) & 1);
+                    s[e] = seen ? s[e] : -INFINITY;
+                }
             }
             float mx = fmaxf(s[0], s[1]);
 #pragma unroll
@@ -645,57 +672,29 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     lrow_sum = M::add2(pf[t].w, lrow_sum);
                 }
             }
-            // A hidden key's weight is 0, and 0 * inf is not: V elements that are not finite leave the
-            // product, and reach the rows that see them through counts of +inf, -inf and NaN.
-            if constexpr (!kQ8) {
-                if (need_mask) {
-                    pa_u16x2 top = {0, 0};
+            // A hidden key's weight is 0, but 0 * inf is not: V elements that are not finite are left out
+            // of the product here, and add_odd gives them to the rows that see them.
+            bool odd_here = false;
+            if constexpr (!kQ8 && kMasked) {
+                pa_u16x2 top = {0, 0};
 #pragma unroll
-                    for (int dt = 0; dt < D / 32; dt++)
+                for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            const uint4 a = kPreV ? va[kPreV ? dt : 0][t] : load_va(dt, t);
+                    for (int t = 0; t < 2; t++) {
+                        const uint4 a = kPreV ? va[kPreV ? dt : 0][t] : load_va(dt, t);
+                        top = __builtin_elementwise_max(top, pa_mag(a.x));
+                        top = __builtin_elementwise_max(top, pa_mag(a.y));
+                        top = __builtin_elementwise_max(top, pa_mag(a.z));
+                        top = __builtin_elementwise_max(top, pa_mag(a.w));
+                    }
+                odd_here = __any(top[0] >= M::kInf || top[1] >= M::kInf);
+                odd |= odd_here;
+                if constexpr (kPreV) {
+                    if (odd_here) {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const uint32_t x = (i == 0 ? a.x : i == 1 ? a.y : i == 2 ? a.z : a.w) & 0x7fff7fffu;
-                                top = __builtin_elementwise_max(top, __builtin_bit_cast(pa_u16x2, x));
-                            }
-                        }
-                    if (__any(top[0] >= M::kInf || top[1] >= M::kInf)) {
+                        for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
-                        for (int dt = 0; dt < D / 32; dt++) {
-                            pa_f32x16 cnt = zero;
-#pragma unroll
-                            for (int t = 0; t < 2; t++) {
-                                const uint4 a = kPreV ? va[kPreV ? dt : 0][t] : load_va(dt, t);
-                                uint32_t fin[4], code[4], see[4];
-#pragma unroll
-                                for (int i = 0; i < 4; i++) {
-                                    const uint32_t x = i == 0 ? a.x : i == 1 ? a.y : i == 2 ? a.z : a.w;
-                                    fin[i] = code[i] = see[i] = 0;
-#pragma unroll
-                                    for (int j = 0; j < 2; j++) {
-                                        const uint32_t h = x >> (16 * j) & 0xffffu, mag = h & 0x7fffu;
-                                        const float what = mag < M::kInf ? 0.0f : mag > M::kInf ? 4096.0f : h >> 15 ? 64.0f : 1.0f;
-                                        if (mag < M::kInf) fin[i] |= h << (16 * j);
-                                        code[i] |= (M::pack2(what, 0.0f) & 0xffffu) << (16 * j);
-                                        if (seen >> (8 * t + 2 * i + j) & 1) see[i] |= (M::pack2(1.0f, 0.0f) & 0xffffu) << (16 * j);
-                                    }
-                                }
-                                o[dt] = M::mma(make_uint4(fin[0], fin[1], fin[2], fin[3]), pf[t], o[dt]);
-                                cnt = M::mma(make_uint4(code[0], code[1], code[2], code[3]),
-                                             make_uint4(see[0], see[1], see[2], see[3]), cnt);
-                            }
-#pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                const int c = (int)cnt[e];
-                                float add = c & 63 ? INFINITY : 0.0f;
-                                if (c >> 6 & 63) add -= INFINITY;
-                                if (c >> 12) add = NAN;
-                                o[dt][e] += add;
-                            }
-                        }
-                        return;
+                            for (int t = 0; t < 2; t++) va[dt][t] = pa_finite<M>(va[dt][t]);
                     }
                 }
             }
@@ -704,17 +703,26 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    const uint4 a = kPreV ? va[kPreV ? dt : 0][t] : load_va(dt, t);
+                    uint4 a = kPreV ? va[kPreV ? dt : 0][t] : load_va(dt, t);
+                    if constexpr (!kPreV && !kQ8 && kMasked) {
+                        if (odd_here) a = pa_finite<M>(a);
+                    }
                     o[dt] = M::mma(a, pf[t], o[dt]);
                 }
             __builtin_amdgcn_s_setprio(0);
         };
         auto compute_tile = [&](const uint16_t* kb, const uint16_t* vb, const float* sc, int t0, unsigned bad) __attribute__((always_inline)) {
+            if (!wave_active) return;
+            if (t0 + BN - 1 <= hi_min && t0 >= lo_max && !bad) {
+#pragma unroll
+                for (int i = 0; i < BN / 32 / KH; i++)
+                    subtile(std::false_type{}, kb, vb, sc, KH * i + kh, t0 + 32 * (KH * i + kh), 0u);
+                return;
+            }
 #pragma unroll 1
             for (int sb = kh; sb < BN / 32; sb += KH) {
                 const int ts = t0 + 32 * sb;
-                if (!(wave_active && ts <= hi_max && ts + 31 >= lo_min)) continue;
-                subtile(kb, vb, sc, sb, ts, bad >> (2 * sb) & 3);
+                if (ts <= hi_max && ts + 31 >= lo_min) subtile(std::true_type{}, kb, vb, sc, sb, ts, bad >> (2 * sb) & 3);
             }
         };
 
@@ -736,9 +744,11 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     bad |= !there;
                 }
                 some_bad = __syncthreads_or(bad);
+                ever_bad |= some_bad;
             }
             if constexpr (kQ8) {
                 load_q8(t_begin);
+                settle_q();
                 if (rt == it0) prepare_q();
                 store_q8(Ks0, Vs0, Sc0);
                 __syncthreads();
@@ -787,6 +797,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     if (n_tiles > 1) dma_tile(t_begin + BN, Ks1, Vs1);
                     if (n_tiles > 2) dma_tile(t_begin + 2 * BN, Ks2, Vs2);
                 }
+                settle_q();
                 for (int it = 0; it < n_tiles; it += NBUF) {
                     step(integral_constant<int, 0>{}, it);
                     if (it + 1 >= n_tiles) break;
@@ -796,6 +807,40 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                         step(integral_constant<int, 2>{}, it + 2);
                         if (it + 3 >= n_tiles) break;
                         step(integral_constant<int, 3>{}, it + 3);
+                    }
+                }
+            }
+        }
+
+        // V elements that are not finite in the sub-tiles where they were left out, a key at a time:
+        // p * inf is inf of that sign for every row that sees the key, two signs or a NaN make NaN.
+        if (!kQ8 && odd) {
+#pragma unroll 1
+            for (int it = it0; it < it1; it++) {
+                const int t0 = blk.t_first + it * BN;
+                const bool full = t0 + BN - 1 <= hi_min && t0 >= lo_max && !(SRC == kPaPages && ever_bad);
+                if (full) continue;
+#pragma unroll 1
+                for (int i = kh * 32; i < BN; i += i % 32 == 31 ? 32 * (KH - 1) + 1 : 1) {
+                    const int key = t0 + i;
+                    if (key > last) break;
+                    int64_t at;
+                    if constexpr (SRC == kPaPacked) {
+                        at = (int64_t)(blk.beg + key) * p.row_stride;
+                    } else {
+                        const int id = p.seqs.page_table[(int64_t)blk.seq * p.seqs.table_stride + (key >> shift)];
+                        if ((unsigned)id >= (unsigned)p.seqs.n_pages) continue;
+                        at = (int64_t)id * p.page_stride + (int64_t)(key & ps1) * p.row_stride;
+                    }
+                    const uint16_t* v = (const uint16_t*)vb0 + at + 4 * lg;
+                    if ((unsigned)(key - my_lo) < my_seen) {
+#pragma unroll
+                        for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) {
+                                const uint16_t x = v[32 * dt + 8 * (e >> 2) + (e & 3)];
+                                if ((x & 0x7fffu) >= M::kInf) o[dt][e] += to_f32<DT>(x);
+                            }
                     }
                 }
             }
@@ -1037,7 +1082,7 @@ struct PaKernels {
     enum Kind { kFew, kMidStream, kMid, kBig };
     static constexpr int kCus = 256;
     template <typename T>
-    static constexpr int ranges = kCus * std::max(1, T::OCC * 4 / T::NW);
+    static constexpr int ranges = kCus * T::kPerCu;
 
     static Kind kind(const PagedAttnLaunch& p) {
         const int64_t group = p.n_heads / p.n_kv_heads;
