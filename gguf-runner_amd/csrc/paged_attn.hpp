@@ -347,7 +347,14 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         return kQ8 ? lane % SCPR * 16 : ((lane % SCPR) ^ pa_swz<D>(r & 15)) * 16;
     };
     const int rsb = (int)p.row_stride * EB;
-    const int swz_k = pa_swz<D>(ln & 15);
+    // K fragments: row ln of a sub-tile, chunk 2 i + lg (byte offsets; opaque, so that they are not
+    // taken apart into parts to be added again for every read)
+    int k_off[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) {
+        k_off[i] = 2 * (ln * D + (((2 * i + lg) ^ pa_swz<D>(ln & 15)) << 3));
+        asm volatile("" : "+v"(k_off[i]));
+    }
     const int gi = lane & 15;
     const int v_chunk = 2 * ((lane >> 4) & 1) + ((gi & 3) >> 1);
     // V^T fragments (ds_read_b64_tr_b16): lane i of a 16-lane group supplies row i / 4, columns
@@ -577,10 +584,9 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             const pa_f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             __builtin_amdgcn_s_setprio(1);
             pa_f32x16 s;
-            const uint16_t* krow = kb + (32 * sb + ln) * D;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) {
-                const uint4 a = *(const uint4*)(krow + (((2 * i + lg) ^ swz_k) << 3));
+                const uint4 a = *(const uint4*)((const char*)kb + 64 * sb * D + k_off[i]);
                 s = M::mma(a, qf[i], i == 0 ? zero : s);
             }
             auto load_va = [&](int dt, int t) __attribute__((always_inline)) {
@@ -594,7 +600,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                 const uint2 hi = __builtin_bit_cast(uint2, part[1]);
                 return make_uint4(lo.x, lo.y, hi.x, hi.y);
             };
-            constexpr bool kPreV = D <= 128;
+            constexpr bool kPreV = D <= 128 && !(kQ8 && RW > 1);
             uint4 va[kPreV ? D / 32 : 1][2];
             if constexpr (kPreV) {
 #pragma unroll
