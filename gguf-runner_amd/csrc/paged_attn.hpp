@@ -69,7 +69,11 @@ struct PaMat<BF16> {
     }
     static __device__ __forceinline__ uint32_t pack2(float lo, float hi) { return pack_bf16x2(lo, hi); }
     static __device__ __forceinline__ float add2(uint32_t w, float c) {
-        return c + (__uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u));
+#if defined(__HIP_DEVICE_COMPILE__)
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pa_bf16x2, w), pa_bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
+#else
+        return c;
+#endif
     }
 };
 
@@ -82,7 +86,7 @@ struct PaTile {
     static constexpr int D = D_, RW = RW_, KH = KH_, BN = BN_, NBUF = NBUF_, OCC = OCC_;
     static constexpr int NW = RW * KH, NT = NW * 64, BM = RW * 32;
     static_assert(BN % (32 * KH) == 0, "every key part has its sub-tiles");
-    static constexpr int kLds = 4 * NBUF * BN * D + 4096 + 24 * BN;  // at most (page ids, Q8 scales)
+    static constexpr int kLds = 4 * NBUF * BN * D + 2048 + 24 * BN + (KH > 1 ? 512 * NW : 0) + 64;  // at most (page ids, Q8 scales, m and l)
     // workgroups a CU holds: by waves, and by its 160 KB of LDS
     static constexpr int kPerCu = OCC * 4 / NW < 163840 / kLds ? (OCC * 4 / NW < 1 ? 1 : OCC * 4 / NW) : 163840 / kLds;
 };
@@ -330,6 +334,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     // Page ids of a run of tiles (-1: not there): read from the table once per run, so that
     // no load of a tile waits for another
     constexpr int kIds = 512;
+    __shared__ float Ml[KH > 1 ? T::NW * 128 : 1];  // the key parts' m and l
     __shared__ int Ids[SRC == kPaPacked ? 1 : kIds];
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -347,28 +352,30 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         return kQ8 ? lane % SCPR * 16 : ((lane % SCPR) ^ pa_swz<D>(r & 15)) * 16;
     };
     const int rsb = (int)p.row_stride * EB;
-    // K fragments: row ln of a sub-tile, chunk 2 i + lg (byte offsets; opaque, so that they are not
-    // taken apart into parts to be added again for every read)
-    int k_off[D / 16];
-#pragma unroll
-    for (int i = 0; i < D / 16; i++) {
-        k_off[i] = 2 * (ln * D + (((2 * i + lg) ^ pa_swz<D>(ln & 15)) << 3));
-        asm volatile("" : "+v"(k_off[i]));
-    }
+    // K fragments: row ln of a sub-tile, chunk 2 i + lg; V^T fragments (ds_read_b64_tr_b16): lane i
+    // of a 16-lane group supplies row i / 4, columns 4 (i % 4) .. +3 of a 4 x 16 block (b) of O^T
+    // tile dt and receives its column i.  Byte offsets, the V ones less where the V arrays start
+    // in LDS (kVAt), which keeps every other part of an address within the instruction's 16-bit
+    // offset.  The chunk number only touches the bits of an offset below the row size, so
+    // offset(i) = offset(0) ^ 32 i and offset(dt) = offset(0) ^ 64 dt.  head_dim 256, which has no
+    // registers to keep them all, makes them where they are used (an xor each); the empty asm
+    // statements keep the compiler from taking offsets apart or moving them out of the loop.
+    constexpr bool kMakeOff = D == 256;
+    constexpr int kVAt = NBUF * BN * D * 2;
     const int gi = lane & 15;
     const int v_chunk = 2 * ((lane >> 4) & 1) + ((gi & 3) >> 1);
-    // V^T fragments (ds_read_b64_tr_b16): lane i of a 16-lane group supplies row i / 4, columns
-    // 4 (i % 4) .. +3 of a 4 x 16 block and receives its column i.  v_off: the byte offset of
-    // O^T tile dt's block b, less where the V arrays start in LDS, which keeps every other
-    // part of the address within the instruction's 16-bit offset.
-    constexpr int kVAt = NBUF * BN * D * 2;
-    int v_off[D / 32][2];
+    int k_off[kMakeOff ? 1 : D / 16], v_off[kMakeOff ? 1 : D / 32][2];
 #pragma unroll
-    for (int dt = 0; dt < D / 32; dt++)
+    for (int i = 0; i < (kMakeOff ? 1 : D / 16); i++) {
+        k_off[i] = (2 * (ln * D + ((lg ^ pa_swz<D>(ln & 15)) << 3))) ^ (32 * i);
+        asm volatile("" : "+v"(k_off[i]));
+    }
+#pragma unroll
+    for (int dt = 0; dt < (kMakeOff ? 1 : D / 32); dt++)
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const int r = 8 * b + 4 * lg + (gi >> 2);
-            v_off[dt][b] = kVAt + 2 * (r * D + (gi & 1) * 4 + (((4 * dt + v_chunk) ^ pa_swz<D>(r & 15)) << 3));
+            v_off[dt][b] = (kVAt + 2 * (r * D + (gi & 1) * 4 + ((v_chunk ^ pa_swz<D>(r & 15)) << 3))) ^ (64 * dt);
             asm volatile("" : "+v"(v_off[dt][b]));
         }
 
@@ -581,19 +588,21 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                            unsigned bad) __attribute__((always_inline)) {
             constexpr bool kMasked = decltype(masked)::value;
             __builtin_amdgcn_sched_barrier(0);  // sub-tiles are not interleaved: the registers hold one
+            if constexpr (kMakeOff) asm volatile("" : "+v"(k_off[0]), "+v"(v_off[0][0]), "+v"(v_off[0][1]));
             const pa_f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             __builtin_amdgcn_s_setprio(1);
             pa_f32x16 s;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) {
-                const uint4 a = *(const uint4*)((const char*)kb + 64 * sb * D + k_off[i]);
+                const uint4 a = *(const uint4*)((const char*)kb + 64 * sb * D + (kMakeOff ? k_off[0] ^ (32 * i) : k_off[kMakeOff ? 0 : i]));
                 s = M::mma(a, qf[i], i == 0 ? zero : s);
             }
             auto load_va = [&](int dt, int t) __attribute__((always_inline)) {
                 pa_i16x4 part[2];
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
-                    const char* at = (const char*)vb - kVAt + (32 * sb + 16 * t) * D * 2 + v_off[dt][b];
+                    const int off = kMakeOff ? v_off[0][b] ^ (64 * dt) : v_off[kMakeOff ? 0 : dt][b];
+                    const char* at = (const char*)vb - kVAt + (32 * sb + 16 * t) * D * 2 + off;
                     part[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GR_PA_LDS pa_i16x4*)at);
                 }
                 const uint2 lo = __builtin_bit_cast(uint2, part[0]);
@@ -642,9 +651,9 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                 lrow_sum *= alpha;
 #pragma unroll
                 for (int dt = 0; dt < D / 32; dt++) {
-                    if constexpr (D == 256) asm volatile("" : "+v"(o[dt]));  // moved to VGPRs here only
+                    if constexpr (D == 256 && T::OCC == 1) asm volatile("" : "+v"(o[dt]));  // moved to VGPRs here only
                     o[dt] *= alpha;
-                    if constexpr (D == 256) asm volatile("" : "+a"(o[dt]));
+                    if constexpr (D == 256 && T::OCC == 1) asm volatile("" : "+a"(o[dt]));
                 }
             }
             float w[16];
@@ -704,15 +713,21 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     }
                 }
             }
+            if constexpr (!kPreV && !kQ8 && kMasked) {
+                if (odd_here) {
+#pragma unroll
+                    for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+                        for (int t = 0; t < 2; t++) o[dt] = M::mma(pa_finite<M>(load_va(dt, t)), pf[t], o[dt]);
+                    return;
+                }
+            }
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    uint4 a = kPreV ? va[kPreV ? dt : 0][t] : load_va(dt, t);
-                    if constexpr (!kPreV && !kQ8 && kMasked) {
-                        if (odd_here) a = pa_finite<M>(a);
-                    }
+                    const uint4 a = kPreV ? va[kPreV ? dt : 0][t] : load_va(dt, t);
                     o[dt] = M::mma(a, pf[t], o[dt]);
                 }
             __builtin_amdgcn_s_setprio(0);
@@ -861,14 +876,16 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         const bool row_ok = row < n_pr;
         const int tok = token_of(row);
         if constexpr (KH > 1) {
-            // Every key part leaves (O, m, l) of its rows in the tile buffers; part k then adds up the
-            // D / 32 / KH (at least one) O^T tiles that are its share: O = sum O_k 2^(m_k - m), m = max m_k.
-            constexpr int NO = D / 32 * 16;
-            static_assert(RW == 1 && KH * NO * 64 * 4 <= 2 * BN * D * 2 && KH * 128 * 4 <= BN * D * 2, "merge buffers");
-            constexpr int NH = BN * D * 2 / 4;  // floats per buffer
-            static_assert(NH % (NO * 64) == 0, "a part's O lies in one buffer");
-            auto part_o = [&](int k) { return (k * NO * 64 < NH ? (float*)Ks0 : (float*)Ks1) + k * NO * 64 % NH; };
-            float* const ml = (float*)Vs0;
+            // Every key part leaves (O, m, l) of its rows in the tile buffers; part k then adds up its
+            // 1 / KH of the row group's O: O = sum O_k 2^(m_k - m), m = max m_k.
+            constexpr int NO = 32 * D;            // floats of a wave's O
+            constexpr int NH = BN * D / 2;        // floats of a buffer
+            static_assert(RW * KH * NO <= 4 * NH && NH % NO == 0 && D / 8 % KH == 0, "merge buffers");
+            auto part_o = [&](int k) __attribute__((always_inline)) {
+                const int x = (k * RW + rw) * NO, i = x / NH;
+                return (float*)(i == 0 ? Ks0 : i == 1 ? Ks1 : i == 2 ? Vs0 : Vs1) + x % NH;
+            };
+            float* const ml = Ml + rw * 128;      // part k's at + k * RW * 128
             __syncthreads();
             float* const mine = part_o(kh);
 #pragma unroll
@@ -877,18 +894,18 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                 for (int j = 0; j < 4; j++)
                     *(float4*)(mine + ((4 * dt + j) * 64 + lane) * 4) =
                         make_float4(o[dt][4 * j + 0], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
-            ml[kh * 128 + lane] = mrow;
-            ml[kh * 128 + 64 + lane] = lsum;
+            ml[kh * RW * 128 + lane] = mrow;
+            ml[kh * RW * 128 + 64 + lane] = lsum;
             __syncthreads();
             float mk[KH];
             mrow = kPaNone;
 #pragma unroll
-            for (int k = 0; k < KH; k++) mk[k] = ml[k * 128 + lane], mrow = fmaxf(mrow, mk[k]);
+            for (int k = 0; k < KH; k++) mk[k] = ml[k * RW * 128 + lane], mrow = fmaxf(mrow, mk[k]);
             lsum = 0.0f;
 #pragma unroll
             for (int k = 0; k < KH; k++) {
                 mk[k] = __builtin_amdgcn_exp2f(mk[k] - mrow);
-                lsum = fmaf(ml[k * 128 + 64 + lane], mk[k], lsum);
+                lsum = fmaf(ml[k * RW * 128 + 64 + lane], mk[k], lsum);
             }
             constexpr int SH = D / 8 / KH;  // float4s of a part's share
 #pragma unroll

@@ -5,7 +5,7 @@
 
 namespace gr {
 
-using K64 = PaKernels<PaTile<64, 1, 4, 128, 4, 1>, PaTile<64, 1, 4, 128, 2, 2>, PaTile<64, 4, 1, 64, 2, 3>, PaTile<64, 8, 1, 128, 2, 2>>;
+using K64 = PaKernels<PaTile<64, 1, 4, 128, 4, 1>, PaTile<64, 1, 4, 128, 2, 2>, PaTile<64, 4, 1, 64, 2, 3>, PaTile<64, 4, 1, 64, 2, 3>>;
 
 bool paged_attn_fits_d64(const PagedAttnLaunch& p) { return K64::fits(p); }
 size_t paged_attn_ws_d64(const PagedAttnLaunch& p) { return K64::ws(p); }

@@ -13,20 +13,23 @@
 namespace gr {
 
 constexpr int kPagedKvThreads = 256;
+constexpr int kPagedKvFull = 1024;  // workgroups from which on a wave takes more rows
 
-// 8 consecutive elements as floats.
-template <typename T>
-__device__ __forceinline__ void pk_load8(const typename T::storage* src, float* x) {
-    const uint4* p = (const uint4*)src;
-    if constexpr (T::bytes == 4) {
-        const uint4 a = p[0], b = p[1];
-        unpack16<T>(a, x);
-        unpack16<T>(b, x + 4);
-    } else {
-        const uint4 a = p[0];
-        unpack16<T>(a, x);
+// 8 consecutive elements as they are stored: 8 (codes), 16 or 32 bytes.
+template <int BYTES>
+struct PkRaw {
+    using V = std::conditional_t<BYTES == 8, uint2, uint4>;
+    V w[BYTES == 32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* p) {
+        w[0] = ((const V*)p)[0];
+        if constexpr (BYTES == 32) w[1] = ((const V*)p)[1];
     }
-}
+    template <typename T>
+    __device__ __forceinline__ void floats(float* x) const {
+        unpack16<T>(w[0], x);
+        if constexpr (BYTES == 32) unpack16<T>(w[1], x + 4);
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ void pk_store8(typename T::storage* dst, const float* x) {
@@ -76,73 +79,122 @@ __device__ __forceinline__ uint32_t pk_code(float x, float inv) {
 
 struct KvQ8 {};
 
-// lanes_per_row lanes (a power of two up to 64) share a row; 64 / lanes_per_row rows a wave.
-template <int D, typename ROWS, typename KV, bool WRITE>
+// lanes_per_row lanes (a power of two up to 64) share a row, 64 / lanes_per_row rows a wave, U
+// times over: the U rows of a lane are requested together.
+template <int D, typename ROWS, typename KV, bool WRITE, int U>
 __global__ __launch_bounds__(kPagedKvThreads) void paged_kv_kernel(const PagedKvLaunch p, const int lanes_per_row) {
     constexpr int CPH = D / 8;  // pieces per head
     constexpr bool q8 = std::is_same_v<KV, KvQ8>;
+    using RT = typename ROWS::storage;
     const int lane = threadIdx.x & 63;
     const int unit = (int)blockIdx.x * (kPagedKvThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rpw = 64 / lanes_per_row;
-    const int first = (unit >> 1) * rpw;  // the wave's first row; units alternate between K and V
+    const int first = (unit >> 1) * rpw * U;  // the wave's first row; units alternate between K and V
     const int which = unit & 1;
     if (first >= p.seqs.n_rows) return;
-    const int row = first + lane / lanes_per_row;
     const int n_pieces = p.n_kv_heads * CPH;
-    // the first sequence a row of this wave may belong to (rows in front of every sequence: -1)
-    const int seq0 = seq_of_row(p.seqs, first);
-    PagedPlace at{-2, 0};
-    if (row < p.seqs.n_rows && row >= p.seqs.row_start[0]) at = pk_place(p.seqs, row, max(seq0, 0));
-    if (seq0 < 0 && first >= p.seqs.row_start[0]) return;  // behind the last sequence
-    if (at.page == -2 || (WRITE && at.page < 0)) return;
-    using RT = typename ROWS::storage;
-    RT* const rows = (RT*)p.rows[which] + (int64_t)row * p.rows_row_stride;
-    const int64_t cell = (int64_t)at.page * p.page_stride + (int64_t)at.row * p.row_stride;
-    const int64_t sc0 = (int64_t)at.page * p.scale_page_stride + (int64_t)at.row * p.scale_row_stride;
+    const int seq0 = seq_of_row(p.seqs, first);  // -1: in front of every sequence, or behind
+    const int row_beg = p.seqs.row_start[0];
+    if (seq0 < 0 && first >= row_beg) return;
+    PagedPlace at[U];
+    const int wave_end = min(first + rpw * U, p.seqs.n_rows);
+    if (seq0 >= 0 && wave_end <= p.seqs.row_start[seq0 + 1]) {
+        // all of one sequence (most waves of long ones): its sizes once, then the rows' page ids together
+        const int end = seq_row(p.seqs, seq0 + 1);
+        const int p0 = seq_len(p.seqs, seq0, 0) - end;  // position less row
+        int id[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int row = min(first + u * rpw + lane / lanes_per_row, p.seqs.n_rows - 1);
+            id[u] = p.seqs.page_table[(int64_t)seq0 * p.seqs.table_stride + (max(p0 + row, 0) >> p.seqs.page_shift)];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int row = first + u * rpw + lane / lanes_per_row;
+            const bool there = p0 + row >= 0 && (unsigned)id[u] < (unsigned)p.seqs.n_pages;
+            at[u].page = row >= p.seqs.n_rows ? -2 : there ? id[u] : -1;
+            at[u].row = (p0 + row) & ((1 << p.seqs.page_shift) - 1);
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int row = first + u * rpw + lane / lanes_per_row;
+            at[u] = PagedPlace{-2, 0};
+            if (row < p.seqs.n_rows && row >= row_beg) at[u] = pk_place(p.seqs, row, max(seq0, 0));
+        }
+    }
     for (int c = lane % lanes_per_row; c < n_pieces; c += lanes_per_row) {
         const int g = c / CPH, i = (c % CPH) * 8;
-        RT* const r = rows + g * p.rows_head_stride + i;
-        const int64_t e = cell + g * p.head_stride + i;
-        float x[8];
-        if constexpr (WRITE) {
-            pk_load8<ROWS>(r, x);
-            if constexpr (q8) {
-                float amax = 0.0f;
+        // every row's piece is requested before the first is used (rows without a place: some valid one)
+        using ST = std::conditional_t<WRITE, ROWS, std::conditional_t<q8, F16, KV>>;
+        PkRaw<WRITE ? ROWS::bytes * 8 : q8 ? 8 : ST::bytes * 8> raw[U];
+        float sc[U];
 #pragma unroll
-                for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(x[j]));
-                // a head's CPH pieces are CPH adjacent lanes (lanes_per_row is a multiple of CPH)
+        for (int u = 0; u < U; u++) {
+            const int row = min(first + u * rpw + lane / lanes_per_row, p.seqs.n_rows - 1);
+            const int64_t page = max(at[u].page, 0);
+            if constexpr (WRITE) {
+                raw[u].load((const RT*)p.rows[which] + (int64_t)row * p.rows_row_stride + g * p.rows_head_stride + i);
+            } else {
+                const int64_t e = page * p.page_stride + (int64_t)at[u].row * p.row_stride + g * p.head_stride + i;
+                if constexpr (q8) {
+                    raw[u].load((const int8_t*)p.pages[which] + e);
+                    sc[u] = p.scale[which][page * p.scale_page_stride + (int64_t)at[u].row * p.scale_row_stride +
+                                           g * p.scale_head_stride];
+                } else {
+                    raw[u].load((const typename ST::storage*)p.pages[which] + e);
+                }
+            }
+        }
+        float x[U][8];
 #pragma unroll
-                for (int m = CPH / 2; m >= 1; m >>= 1) amax = fmaxf(amax, shfl_xor(amax, m));
-                if (amax < kQ8Least) amax = 0.0f;
-                const float inv = amax == 0.0f ? 0.0f : __fdiv_rn(1.0f, amax) * 127.0f;
-                uint32_t w0 = 0, w1 = 0;
+        for (int u = 0; u < U; u++) {
+            if constexpr (!WRITE && q8) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    w0 |= pk_code(x[j], inv) << (8 * j);
-                    w1 |= pk_code(x[j + 4], inv) << (8 * j);
-                }
-                *(uint2*)((int8_t*)p.pages[which] + e) = make_uint2(w0, w1);
-                if (i == 0)
-                    p.scale[which][sc0 + g * p.scale_head_stride] = amax == 0.0f ? 1.0f : amax * (1.0f / 127.0f);
-            } else {
-                pk_store8<KV>((typename KV::storage*)p.pages[which] + e, x);
-            }
-        } else {
-            if (at.page < 0) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = 0.0f;
-            } else if constexpr (q8) {
-                const uint2 w = *(const uint2*)((const int8_t*)p.pages[which] + e);
-                const float s = p.scale[which][sc0 + g * p.scale_head_stride];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    x[j] = (float)(int8_t)(w.x >> (8 * j)) * s;
-                    x[j + 4] = (float)(int8_t)(w.y >> (8 * j)) * s;
+                    x[u][j] = (float)(int8_t)(raw[u].w[0].x >> (8 * j)) * sc[u];
+                    x[u][j + 4] = (float)(int8_t)(raw[u].w[0].y >> (8 * j)) * sc[u];
                 }
             } else {
-                pk_load8<KV>((const typename KV::storage*)p.pages[which] + e, x);
+                raw[u].template floats<ST>(x[u]);
             }
-            pk_store8<ROWS>(r, x);
+            if (at[u].page < 0) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[u][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int row = first + u * rpw + lane / lanes_per_row;
+            if constexpr (!WRITE) {
+                if (at[u].page != -2)
+                    pk_store8<ROWS>((RT*)p.rows[which] + (int64_t)row * p.rows_row_stride + g * p.rows_head_stride + i, x[u]);
+            } else {
+                const int64_t e = (int64_t)at[u].page * p.page_stride + (int64_t)at[u].row * p.row_stride + g * p.head_stride + i;
+                if constexpr (q8) {
+                    float amax = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(x[u][j]));
+                    // a head's CPH pieces are CPH adjacent lanes (lanes_per_row is a multiple of CPH)
+#pragma unroll
+                    for (int m = CPH / 2; m >= 1; m >>= 1) amax = fmaxf(amax, shfl_xor(amax, m));
+                    if (at[u].page < 0) continue;
+                    if (amax < kQ8Least) amax = 0.0f;
+                    const float inv = amax == 0.0f ? 0.0f : __fdiv_rn(1.0f, amax) * 127.0f;
+                    uint32_t w0 = 0, w1 = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        w0 |= pk_code(x[u][j], inv) << (8 * j);
+                        w1 |= pk_code(x[u][j + 4], inv) << (8 * j);
+                    }
+                    *(uint2*)((int8_t*)p.pages[which] + e) = make_uint2(w0, w1);
+                    if (i == 0)
+                        p.scale[which][(int64_t)at[u].page * p.scale_page_stride + (int64_t)at[u].row * p.scale_row_stride +
+                                       g * p.scale_head_stride] = amax == 0.0f ? 1.0f : amax * (1.0f / 127.0f);
+                } else if (at[u].page >= 0) {
+                    pk_store8<KV>((typename KV::storage*)p.pages[which] + e, x[u]);
+                }
+            }
         }
     }
 }
@@ -152,9 +204,16 @@ static hipError_t launch_kv(const PagedKvLaunch& p, hipStream_t st) {
     const int pieces = p.n_kv_heads * (D / 8);
     int lpr = 64;
     while (lpr > D / 8 && lpr / 2 >= pieces) lpr /= 2;
-    const int64_t units = 2 * (((int64_t)p.seqs.n_rows + 64 / lpr - 1) / (64 / lpr));
-    const int64_t wgs = (units + kPagedKvThreads / 64 - 1) / (kPagedKvThreads / 64);
-    paged_kv_kernel<D, ROWS, KV, WRITE><<<dim3((unsigned)wgs), kPagedKvThreads, 0, st>>>(p, lpr);
+    auto wgs = [&](int rows) {  // for waves of that many rows
+        const int64_t units = 2 * (((int64_t)p.seqs.n_rows + rows - 1) / rows);
+        return (units + kPagedKvThreads / 64 - 1) / (kPagedKvThreads / 64);
+    };
+    constexpr int U = 4;
+    const int rows = 64 / lpr;
+    if (wgs(rows * U) >= kPagedKvFull)
+        paged_kv_kernel<D, ROWS, KV, WRITE, U><<<dim3((unsigned)wgs(rows * U)), kPagedKvThreads, 0, st>>>(p, lpr);
+    else
+        paged_kv_kernel<D, ROWS, KV, WRITE, 1><<<dim3((unsigned)wgs(rows)), kPagedKvThreads, 0, st>>>(p, lpr);
     return hipGetLastError();
 }
 
