@@ -1,6 +1,4 @@
 // Attention over pages and packed rows: dispatch by head_dim (paged_attn.hpp).
-#include <algorithm>
-
 #include "paged_attn.hpp"
 
 namespace gr {

@@ -25,6 +25,8 @@
 // divides leaves unnormalised partials (O, m, l) which paged_combine_kernel joins.
 #pragma once
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "gr_common.hpp"
@@ -317,20 +319,20 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     constexpr int RPV = 64 / SCPR;          // ... of a wave: inside one run of 16 rows, so one page
     constexpr int EB = kQ8 ? 1 : 2;         // bytes per stored element
     static_assert(LD >= 1 && LD <= 32 && BN * SCPR % NT == 0 && BN / 16 <= 32 && BN <= NT, "tile shape");
-    static_assert(NBUF == 2 || (NBUF == 4 && !kQ8), "buffers");
+    static_assert(kQ8 ? NBUF <= 2 : NBUF == 2 || NBUF == 4, "buffers");
 
     // distinct arrays, so that the compiler sees that filling one never aliases reading another
     __shared__ __attribute__((aligned(16))) uint16_t Ks0[BN * D];
-    __shared__ __attribute__((aligned(16))) uint16_t Ks1[BN * D];
+    __shared__ __attribute__((aligned(16))) uint16_t Ks1[NBUF > 1 ? BN * D : 8];
     __shared__ __attribute__((aligned(16))) uint16_t Vs0[BN * D];
-    __shared__ __attribute__((aligned(16))) uint16_t Vs1[BN * D];
+    __shared__ __attribute__((aligned(16))) uint16_t Vs1[NBUF > 1 ? BN * D : 8];
     __shared__ __attribute__((aligned(16))) uint16_t Ks2[NBUF == 4 ? BN * D : 8];
     __shared__ __attribute__((aligned(16))) uint16_t Ks3[NBUF == 4 ? BN * D : 8];
     __shared__ __attribute__((aligned(16))) uint16_t Vs2[NBUF == 4 ? BN * D : 8];
     __shared__ __attribute__((aligned(16))) uint16_t Vs3[NBUF == 4 ? BN * D : 8];
     // Q8: c * k_scale, log2 v_scale, 1 / v_scale of the tile's keys
     __shared__ __attribute__((aligned(16))) float Sc0[kQ8 ? 3 * BN : 4];
-    __shared__ __attribute__((aligned(16))) float Sc1[kQ8 ? 3 * BN : 4];
+    __shared__ __attribute__((aligned(16))) float Sc1[kQ8 && NBUF > 1 ? 3 * BN : 4];
     // Page ids of a run of tiles (-1: not there): read from the table once per run, so that
     // no load of a tile waits for another
     constexpr int kIds = 512;
@@ -773,7 +775,18 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                 if (rt == it0) prepare_q();
                 store_q8(Ks0, Vs0, Sc0);
                 __syncthreads();
-                for (int it = 0; it < n_tiles; it += 2) {
+                // the next tile's codes are on their way to registers while this one is used; one tile in
+                // LDS takes two barriers a tile, but leaves room for other workgroups
+                for (int it = 0; NBUF == 1 && it < n_tiles; it++) {
+                    const int t0 = t_begin + it * BN;
+                    if (it + 1 < n_tiles) load_q8(t0 + BN);
+                    compute_tile(Ks0, Vs0, Sc0, t0, bad_runs(t0));
+                    if (it + 1 >= n_tiles) break;
+                    __syncthreads();
+                    store_q8(Ks0, Vs0, Sc0);
+                    __syncthreads();
+                }
+                for (int it = 0; NBUF == 2 && it < n_tiles; it += 2) {
                     const int t0 = t_begin + it * BN;
                     if (it + 1 < n_tiles) load_q8(t0 + BN);
                     compute_tile(Ks0, Vs0, Sc0, t0, bad_runs(t0));
@@ -880,10 +893,11 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             // 1 / KH of the row group's O: O = sum O_k 2^(m_k - m), m = max m_k.
             constexpr int NO = 32 * D;            // floats of a wave's O
             constexpr int NH = BN * D / 2;        // floats of a buffer
-            static_assert(RW * KH * NO <= 4 * NH && NH % NO == 0 && D / 8 % KH == 0, "merge buffers");
+            static_assert(RW * KH * NO <= 2 * NBUF * NH && NH % NO == 0 && D / 8 % KH == 0, "merge buffers");
             auto part_o = [&](int k) __attribute__((always_inline)) {
                 const int x = (k * RW + rw) * NO, i = x / NH;
-                return (float*)(i == 0 ? Ks0 : i == 1 ? Ks1 : i == 2 ? Vs0 : Vs1) + x % NH;
+                if constexpr (NBUF == 1) return (float*)(i == 0 ? Ks0 : Vs0) + x % NH;
+                else return (float*)(i == 0 ? Ks0 : i == 1 ? Ks1 : i == 2 ? Vs0 : Vs1) + x % NH;
             };
             float* const ml = Ml + rw * 128;      // part k's at + k * RW * 128
             __syncthreads();
@@ -1098,39 +1112,72 @@ hipError_t launch_paged_attn_d64(const PagedAttnLaunch& p, hipStream_t st);
 hipError_t launch_paged_attn_d128(const PagedAttnLaunch& p, hipStream_t st);
 hipError_t launch_paged_attn_d256(const PagedAttnLaunch& p, hipStream_t st);
 
+// What a kernel's workgroup takes for a tile, us measured on MI355X: alone on its CU, and of
+// the CU's time when the CU is full.
+struct PaTime {
+    float alone, shared;
+};
+
 // The kernels of a head_dim and which of them a call takes.  Few: blocks of few rows, key
-// parts (FewQ8 over Q8 pages); Mid, Big: whole row blocks.
-template <typename Few, typename FewQ8, typename Mid, typename Big>
+// parts (FewQ8 over Q8 pages), always cut; Mid, Big: one block per workgroup (tMid, tBig), or
+// Cut (its t and what cutting costs, joining included): the tiles of all blocks in equal ranges.
+// Costs: kMid, kBig, kCut, kCutFixed.
+template <typename Few, typename FewQ8, typename Mid, typename Big, typename Cut, typename Costs>
 struct PaKernels {
-    enum Kind { kFew, kMidStream, kMid, kBig };
+    enum Kind { kFew, kMid, kBig, kCut };
     static constexpr int kCus = 256;
     template <typename T>
     static constexpr int ranges = kCus * T::kPerCu;
 
+    // Uncut, a launch lasts as long as its longest block alone, or as its tiles take on full CUs,
+    // whole rounds of workgroups where all blocks are about as long and one does not hold them; cut, as its places
+    // (each block counts its sequence's longest) and the join.
     static Kind kind(const PagedAttnLaunch& p) {
-        const int64_t group = p.n_heads / p.n_kv_heads;
+        const int group = p.n_heads / p.n_kv_heads;
         if (std::min<int64_t>(p.max_rows, p.seqs.n_rows) * group <= Few::BM) return kFew;
-        const int64_t rows = (int64_t)p.seqs.n_rows * group * p.n_kv_heads;
-        if (rows >= (int64_t)2 * kCus * Big::BM) return kBig;
-        if (rows >= (int64_t)2 * kCus * Mid::BM) return kMid;
-        return kMidStream;
+        const double len = std::min(p.max_len, p.seqs.max_len), rows = std::min<double>(p.max_rows, len);
+        const bool even = p.window > 0 ? len > 2.0 * p.window : rows < 0.4 * len;
+        auto blocks = [&](int bm) {  // half of every sequence's last block is empty
+            return ((double)p.seqs.n_rows * group / bm + 0.5 * std::min(p.seqs.n_seq, p.seqs.n_rows)) * p.n_kv_heads;
+        };
+        auto tiles = [&](double keys, int bm, int bn) {
+            return p.window > 0 ? std::min(keys / bn, (double)(p.window + bm / group) / bn + 1) : keys / bn;
+        };
+        auto uncut = [&](auto t, PaTime c) {
+            using T = decltype(t);
+            double n = blocks(T::BM);
+            if (even && n > ranges<T>) n = std::ceil(n / ranges<T>) * ranges<T>;
+            return std::max(tiles(len, T::BM, T::BN) * c.alone,
+                            n * tiles(len - rows / 2, T::BM, T::BN) * c.shared / kCus);
+        };
+        const double mid = uncut(Mid{}, Costs::kMid), big = uncut(Big{}, Costs::kBig);
+        const double cut = Costs::kCutFixed + blocks(Cut::BM) * tiles(len, Cut::BM, Cut::BN) * Costs::kCut.shared / kCus;
+        return cut < std::min(mid, big) ? kCut : big < mid ? kBig : kMid;
+    }
+    // Workgroups of a stream launch: what the GPU holds at once, or the places there are by the
+    // caller's bounds, in eights.
+    template <typename T>
+    static int n_ranges(const PagedAttnLaunch& p) {
+        const int64_t tiles = (std::min(p.max_len, p.seqs.max_len) + T::BN - 1) / T::BN;
+        const int64_t places = pa_max_blocks<T>(p) * p.n_kv_heads * std::max<int64_t>(tiles, 1);
+        return (int)std::min<int64_t>(ranges<T>, (places + 7) / 8 * 8);
     }
     static size_t ws(const PagedAttnLaunch& p) {
         switch (kind(p)) {
-            case kFew: return p.kv_dtype == GR_DTYPE_Q8 ? pa_ws_bytes<FewQ8>(ranges<FewQ8>) : pa_ws_bytes<Few>(ranges<Few>);
-            case kMidStream: return pa_ws_bytes<Mid>(ranges<Mid>);
+            case kFew: return p.kv_dtype == GR_DTYPE_Q8 ? pa_ws_bytes<FewQ8>(n_ranges<FewQ8>(p)) : pa_ws_bytes<Few>(n_ranges<Few>(p));
+            case kCut: return pa_ws_bytes<Cut>(n_ranges<Cut>(p));
             default: return 256;
         }
     }
     static bool fits(const PagedAttnLaunch& p) {
-        return std::max({pa_max_places<Few>(p), pa_max_places<FewQ8>(p), pa_max_places<Mid>(p)}) < INT32_MAX;
+        return std::max({pa_max_places<Few>(p), pa_max_places<FewQ8>(p), pa_max_places<Cut>(p)}) < INT32_MAX;
     }
     template <typename DT, int SRC>
     static hipError_t launch(const PagedAttnLaunch& p, hipStream_t st) {
         using F = std::conditional_t<SRC == kPaPagesQ8, FewQ8, Few>;
         switch (kind(p)) {
-            case kFew: return pa_launch_stream<DT, F, SRC>(p, ranges<F>, 1, st);
-            case kMidStream: return pa_launch_stream<DT, Mid, SRC>(p, ranges<Mid>, 1, st);
+            case kFew: return pa_launch_stream<DT, F, SRC>(p, n_ranges<F>(p), 1, st);
+            case kCut: return pa_launch_stream<DT, Cut, SRC>(p, n_ranges<Cut>(p), 1, st);
             case kMid: return pa_launch_ordered<DT, Mid, SRC>(p, st);
             default: return pa_launch_ordered<DT, Big, SRC>(p, st);
         }

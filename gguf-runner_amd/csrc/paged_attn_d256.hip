@@ -1,11 +1,14 @@
 // head_dim 256 of the attention over pages and packed rows (paged_attn.hpp).
-#include <algorithm>
-
 #include "paged_attn.hpp"
 
 namespace gr {
 
-using K256 = PaKernels<PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 4, 1, 64, 2, 1>, PaTile<256, 4, 1, 64, 2, 1>>;
+struct Costs256 {
+    static constexpr PaTime kMid{2.5f, 2.5f}, kBig{3.3f, 3.2f}, kCut{3.6f, 3.6f};
+    static constexpr float kCutFixed = 24.0f;
+};
+using K256 = PaKernels<PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 2, 2, 64, 2, 1>,
+                       PaTile<256, 4, 1, 64, 2, 1>, PaTile<256, 4, 1, 64, 2, 1>, Costs256>;
 
 bool paged_attn_fits_d256(const PagedAttnLaunch& p) { return K256::fits(p); }
 size_t paged_attn_ws_d256(const PagedAttnLaunch& p) { return K256::ws(p); }

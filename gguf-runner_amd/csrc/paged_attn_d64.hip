@@ -1,11 +1,14 @@
 // head_dim 64 of the attention over pages and packed rows (paged_attn.hpp).
-#include <algorithm>
-
 #include "paged_attn.hpp"
 
 namespace gr {
 
-using K64 = PaKernels<PaTile<64, 1, 4, 128, 4, 1>, PaTile<64, 1, 4, 128, 2, 2>, PaTile<64, 4, 1, 64, 2, 3>, PaTile<64, 4, 1, 64, 2, 3>>;
+struct Costs64 {
+    static constexpr PaTime kMid{1.0f, 0.74f}, kBig{1.0f, 0.74f}, kCut{2.4f, 2.4f};
+    static constexpr float kCutFixed = 18.0f;
+};
+using K64 = PaKernels<PaTile<64, 1, 4, 128, 2, 2>, PaTile<64, 1, 4, 128, 2, 2>, PaTile<64, 4, 1, 64, 2, 3>, PaTile<64, 4, 1, 64, 2, 3>,
+                      PaTile<64, 8, 1, 128, 2, 2>, Costs64>;
 
 bool paged_attn_fits_d64(const PagedAttnLaunch& p) { return K64::fits(p); }
 size_t paged_attn_ws_d64(const PagedAttnLaunch& p) { return K64::ws(p); }
