@@ -79,6 +79,7 @@ struct PaMat<BF16> {
     }
 };
 
+enum PaMode { kPaFull, kPaMasked, kPaEither };
 enum PaSrc { kPaPacked = 0, kPaPages = 1, kPaPagesQ8 = 2 };
 
 // Tiles of a kernel: RW row groups x KH key parts, BN keys, NBUF tiles in LDS (NBUF - 1 of
@@ -130,6 +131,21 @@ template <int D>
 __device__ __forceinline__ int pa_swz(int r) {
     if constexpr (D == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
     else return ((r << 2) ^ (r << 1) ^ (r >> 2)) & 15;
+}
+
+// Asks the scheduler for this order of the products in front of it: the LDS reads of the first
+// four (READS each), then a product and the reads of the one four later, so that a single wave
+// does not wait for every read.
+template <int N, int READS>
+__device__ __forceinline__ void pa_pipeline() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4 * READS, 0);
+#pragma unroll
+    for (int i = 0; i < N - 4; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // 8 int8 codes -> 8 exact f16: sign bit flipped, u = code + 128 becomes the f16 1024 + u
@@ -200,6 +216,7 @@ struct PaBlock {
     int beg, n, p0;           // first row, rows, position of the first row
     int nb, vt;
     int t_first, kend;        // keys [.., kend); tiles start at t_first
+    int all_lo, all_hi;       // every row sees keys all_lo .. all_hi (as far as their pages are there)
     int n_tiles;
 };
 template <int BM, int BN>
@@ -208,6 +225,8 @@ __device__ __forceinline__ void pa_keys(const PagedAttnLaunch& p, PaBlock& b) {
     const int tok0 = b.rb * BM / group, tok1 = (min((b.rb + 1) * BM, b.n * group) - 1) / group;
     b.kend = max(b.p0 + tok1 + 1, 0);
     const int lo = p.window > 0 ? max(b.p0 + tok0 + 1 - p.window, 0) : 0;
+    b.all_lo = p.window > 0 ? max(b.p0 + tok1 + 1 - p.window, 0) : 0;
+    b.all_hi = b.p0 + tok0;
     b.t_first = lo / BN * BN;
     b.n_tiles = b.kend > b.t_first ? (b.kend - b.t_first + BN - 1) / BN : 0;
 }
@@ -362,7 +381,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     // offset(i) = offset(0) ^ 32 i and offset(dt) = offset(0) ^ 64 dt.  head_dim 256, which has no
     // registers to keep them all, makes them where they are used (an xor each); the empty asm
     // statements keep the compiler from taking offsets apart or moving them out of the loop.
-    constexpr bool kMakeOff = D == 256;
+    constexpr bool kMakeOff = D == 256, kEither = D == 256;
     constexpr int kVAt = NBUF * BN * D * 2;
     const int gi = lane & 15;
     const int v_chunk = 2 * ((lane >> 4) & 1) + ((gi & 3) >> 1);
@@ -581,14 +600,16 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
 #pragma unroll
             for (int e = 0; e < 16; e++) o[dt][e] = 0.0f;
         float mrow = kPaNone, lrow_sum = 0.0f;
-        bool odd = false;  // some partly hidden sub-tile has V elements that are not finite
+        bool odd = false;  // V elements that are not finite were left out of some tile
         const float c2 = p.scale_log2;
 
-        // One 32-key sub-tile: keys ts .. ts + 31, rows 32 sb .. of the tile; masked: some row of
-        // the wave does not see all of them (bad: its two 16-key runs that are not there).
-        auto subtile = [&](auto masked, const uint16_t* kb, const uint16_t* vb, const float* sc, int sb, int ts,
+        // One 32-key sub-tile: keys ts .. ts + 31, rows 32 sb .. of the tile; mode kPaFull: every row of
+        // the wave sees all of them, kPaMasked: some do not (bad: its two 16-key runs that are not
+        // there), kPaEither: decided here (one body for both, where O cannot change its registers).
+        auto subtile = [&](auto mode, const uint16_t* kb, const uint16_t* vb, const float* sc, int sb, int ts,
                            unsigned bad) __attribute__((always_inline)) {
-            constexpr bool kMasked = decltype(masked)::value;
+            constexpr bool kMasked = decltype(mode)::value != kPaFull;
+            const bool need = decltype(mode)::value == kPaMasked || ts + 31 > hi_min || ts < lo_max || bad;
             __builtin_amdgcn_sched_barrier(0);  // sub-tiles are not interleaved: the registers hold one
             if constexpr (kMakeOff) asm volatile("" : "+v"(k_off[0]), "+v"(v_off[0][0]), "+v"(v_off[0][1]));
             const pa_f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -596,15 +617,19 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             pa_f32x16 s;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) {
-                const uint4 a = *(const uint4*)((const char*)kb + 64 * sb * D + (kMakeOff ? k_off[0] ^ (32 * i) : k_off[kMakeOff ? 0 : i]));
+                const uint4 a = *(const uint4*)((const char*)kb + (kMakeOff ? (k_off[0] + 64 * sb * D) ^ (32 * i) : 64 * sb * D + k_off[kMakeOff ? 0 : i]));
                 s = M::mma(a, qf[i], i == 0 ? zero : s);
+            }
+            if constexpr (D == 256) {
+                pa_pipeline<D / 16, 1>();
+                asm volatile("" : "+v"(s));
             }
             auto load_va = [&](int dt, int t) __attribute__((always_inline)) {
                 pa_i16x4 part[2];
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
-                    const int off = kMakeOff ? v_off[0][b] ^ (64 * dt) : v_off[kMakeOff ? 0 : dt][b];
-                    const char* at = (const char*)vb - kVAt + (32 * sb + 16 * t) * D * 2 + off;
+                    const int off = kMakeOff ? (v_off[0][b] + 64 * sb * D) ^ (64 * dt) : 64 * sb * D + v_off[kMakeOff ? 0 : dt][b];
+                    const char* at = (const char*)vb - kVAt + 32 * t * D + off;
                     part[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((GR_PA_LDS pa_i16x4*)at);
                 }
                 const uint2 lo = __builtin_bit_cast(uint2, part[0]);
@@ -634,13 +659,16 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                 }
             }
             if constexpr (kMasked) {
-                const int k0 = ts + 4 * lg - my_lo;
+                if (need) {
+                    const int k0 = ts + 4 * lg - my_lo;
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const bool seen = (unsigned)(k0 + 8 * (e >> 2) + (e & 3)) < my_seen && !(bad >> (e >> 3) & 1);
-                    s[e] = seen ? s[e] : -INFINITY;
+                    for (int e = 0; e < 16; e++) {
+                        const bool seen = (unsigned)(k0 + 8 * (e >> 2) + (e & 3)) < my_seen && !(bad >> (e >> 3) & 1);
+                        s[e] = seen ? s[e] : -INFINITY;
+                    }
                 }
             }
+            if constexpr (D == 256) asm volatile("" : "+v"(s));
             float mx = fmaxf(s[0], s[1]);
 #pragma unroll
             for (int e = 2; e < 16; e++) mx = fmaxf(mx, s[e]);
@@ -689,41 +717,6 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     lrow_sum = M::add2(pf[t].w, lrow_sum);
                 }
             }
-            // A hidden key's weight is 0, but 0 * inf is not: V elements that are not finite are left out
-            // of the product here, and add_odd gives them to the rows that see them.
-            bool odd_here = false;
-            if constexpr (!kQ8 && kMasked) {
-                pa_u16x2 top = {0, 0};
-#pragma unroll
-                for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        const uint4 a = kPreV ? va[kPreV ? dt : 0][t] : load_va(dt, t);
-                        top = __builtin_elementwise_max(top, pa_mag(a.x));
-                        top = __builtin_elementwise_max(top, pa_mag(a.y));
-                        top = __builtin_elementwise_max(top, pa_mag(a.z));
-                        top = __builtin_elementwise_max(top, pa_mag(a.w));
-                    }
-                odd_here = __any(top[0] >= M::kInf || top[1] >= M::kInf);
-                odd |= odd_here;
-                if constexpr (kPreV) {
-                    if (odd_here) {
-#pragma unroll
-                        for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-                            for (int t = 0; t < 2; t++) va[dt][t] = pa_finite<M>(va[dt][t]);
-                    }
-                }
-            }
-            if constexpr (!kPreV && !kQ8 && kMasked) {
-                if (odd_here) {
-#pragma unroll
-                    for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-                        for (int t = 0; t < 2; t++) o[dt] = M::mma(pa_finite<M>(load_va(dt, t)), pf[t], o[dt]);
-                    return;
-                }
-            }
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int dt = 0; dt < D / 32; dt++)
@@ -732,21 +725,47 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     const uint4 a = kPreV ? va[kPreV ? dt : 0][t] : load_va(dt, t);
                     o[dt] = M::mma(a, pf[t], o[dt]);
                 }
+            if constexpr (D == 256) pa_pipeline<D / 16, 2>();
             __builtin_amdgcn_s_setprio(0);
         };
         auto compute_tile = [&](const uint16_t* kb, const uint16_t* vb, const float* sc, int t0, unsigned bad) __attribute__((always_inline)) {
             if (!wave_active) return;
-            if (t0 + BN - 1 <= hi_min && t0 >= lo_max && !bad) {
+            using std::integral_constant;
+            if (!kEither && t0 + BN - 1 <= hi_min && t0 >= lo_max && !bad) {
 #pragma unroll
                 for (int i = 0; i < BN / 32 / KH; i++)
-                    subtile(std::false_type{}, kb, vb, sc, KH * i + kh, t0 + 32 * (KH * i + kh), 0u);
+                    subtile(integral_constant<int, kPaFull>{}, kb, vb, sc, KH * i + kh, t0 + 32 * (KH * i + kh), 0u);
                 return;
             }
-#pragma unroll 1
+#pragma unroll(kEither ? BN / 32 / KH : 1)
             for (int sb = kh; sb < BN / 32; sb += KH) {
                 const int ts = t0 + 32 * sb;
-                if (ts <= hi_max && ts + 31 >= lo_min) subtile(std::true_type{}, kb, vb, sc, sb, ts, bad >> (2 * sb) & 3);
+                if (ts <= hi_max && ts + 31 >= lo_min)
+                    subtile(integral_constant<int, kEither ? kPaEither : kPaMasked>{}, kb, vb, sc, sb, ts, bad >> (2 * sb) & 3);
             }
+        };
+
+        // Whether some row of the block does not see every key of the tile.
+        auto partly = [&](int t0, bool bad) __attribute__((always_inline)) {
+            return t0 + BN - 1 > blk.all_hi || t0 < blk.all_lo || bad;
+        };
+        // A hidden key's weight is 0, but 0 * inf is not: V elements of a partly hidden tile that are not
+        // finite become zeros (each thread looks at what it brought), and the rows that see them get
+        // them after the last tile.  Called by the whole workgroup, the tile is in LDS.
+        auto finite_only = [&](uint16_t* vd) __attribute__((always_inline)) {
+            uint4* const mine = (uint4*)(vd + (wave * 64 + lane) * 8);
+            pa_u16x2 top = {0, 0};
+#pragma unroll
+            for (int u = 0; u < LD; u++) {
+                const uint4 a = mine[u * NT];
+                top = __builtin_elementwise_max(top, __builtin_elementwise_max(pa_mag(a.x), pa_mag(a.y)));
+                top = __builtin_elementwise_max(top, __builtin_elementwise_max(pa_mag(a.z), pa_mag(a.w)));
+            }
+            if (!__syncthreads_or(top[0] >= M::kInf || top[1] >= M::kInf)) return;
+            odd = true;
+#pragma unroll 1
+            for (int u = 0; u < LD; u++) mine[u * NT] = pa_finite<M>(mine[u * NT]);
+            __syncthreads();
         };
 
         // The tiles, run of page ids by run.
@@ -823,7 +842,9 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     if (it + NBUF - 1 < n_tiles)
                         dma_tile(t0 + (NBUF - 1) * BN, kbuf(std::integral_constant<int, I + NBUF - 1>{}),
                                  vbuf(std::integral_constant<int, I + NBUF - 1>{}));
-                    compute_tile(kbuf(i), vbuf(i), Sc0, t0, bad_runs(t0));
+                    const unsigned bad = bad_runs(t0);
+                    if (partly(t0, bad)) finite_only(vbuf(i));
+                    compute_tile(kbuf(i), vbuf(i), Sc0, t0, bad);
                 };
                 using std::integral_constant;
                 dma_tile(t_begin, Ks0, Vs0);
@@ -846,16 +867,16 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             }
         }
 
-        // V elements that are not finite in the sub-tiles where they were left out, a key at a time:
-        // p * inf is inf of that sign for every row that sees the key, two signs or a NaN make NaN.
+        // V elements that are not finite, left out of the partly hidden tiles, a key at a time: p * inf is
+        // inf of that sign for every row that sees the key, two signs or a NaN make NaN.  With key
+        // parts, part k takes its keys of every tile.
         if (!kQ8 && odd) {
 #pragma unroll 1
             for (int it = it0; it < it1; it++) {
                 const int t0 = blk.t_first + it * BN;
-                const bool full = t0 + BN - 1 <= hi_min && t0 >= lo_max && !(SRC == kPaPages && ever_bad);
-                if (full) continue;
+                if (!partly(t0, SRC == kPaPages && ever_bad)) continue;
 #pragma unroll 1
-                for (int i = kh * 32; i < BN; i += i % 32 == 31 ? 32 * (KH - 1) + 1 : 1) {
+                for (int i = kh; i < BN; i += KH) {
                     const int key = t0 + i;
                     if (key > last) break;
                     int64_t at;
