@@ -1133,10 +1133,10 @@ hipError_t launch_paged_attn_d64(const PagedAttnLaunch& p, hipStream_t st);
 hipError_t launch_paged_attn_d128(const PagedAttnLaunch& p, hipStream_t st);
 hipError_t launch_paged_attn_d256(const PagedAttnLaunch& p, hipStream_t st);
 
-// What a kernel's workgroup takes for a tile, us measured on MI355X: alone on its CU, and of
-// the CU's time when the CU is full.
+// What a kernel's workgroup takes, us measured on MI355X: for a tile alone on its CU, for a tile
+// of the CU's time when the CU is full, and of that for its start and end.
 struct PaTime {
-    float alone, shared;
+    float alone, shared, start;
 };
 
 // The kernels of a head_dim and which of them a call takes.  Few: blocks of few rows, key
@@ -1167,9 +1167,9 @@ struct PaKernels {
         auto uncut = [&](auto t, PaTime c) {
             using T = decltype(t);
             double n = blocks(T::BM);
-            if (even && n > ranges<T>) n = std::ceil(n / ranges<T>) * ranges<T>;
+            if (even && n > ranges<T>) n = std::ceil(n / ranges<T> - 0.15) * ranges<T>;
             return std::max(tiles(len, T::BM, T::BN) * c.alone,
-                            n * tiles(len - rows / 2, T::BM, T::BN) * c.shared / kCus);
+                            n * (tiles(len - rows / 2, T::BM, T::BN) * c.shared + c.start) / kCus);
         };
         const double mid = uncut(Mid{}, Costs::kMid), big = uncut(Big{}, Costs::kBig);
         const double cut = Costs::kCutFixed + blocks(Cut::BM) * tiles(len, Cut::BM, Cut::BN) * Costs::kCut.shared / kCus;

@@ -4,7 +4,7 @@
 namespace gr {
 
 struct Costs256 {
-    static constexpr PaTime kMid{2.5f, 2.5f}, kBig{3.3f, 3.2f}, kCut{3.6f, 3.6f};
+    static constexpr PaTime kMid{2.0f, 1.75f, 11.0f}, kBig{3.05f, 2.6f, 11.0f}, kCut{3.0f, 3.0f, 0.0f};
     static constexpr float kCutFixed = 24.0f;
 };
 using K256 = PaKernels<PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 2, 2, 64, 2, 1>,
