@@ -992,7 +992,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
 }
 
 // Joins the pieces of the block that boundary w (the start of range w) is the first to cut;
-// blockIdx.y: a row group of it.  Thread (row, 4 elements) runs over the pieces; with few rows
+// blockIdx.y: a row group of it, blockIdx.z: a share of its rows' elements.  Thread (row, 4 elements) runs over the pieces; with few rows
 // the workgroup's spare threads share a row's pieces among them and add up in LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunch p, const int n_ranges) {
@@ -1025,7 +1025,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunc
     while (n_items * parts * 2 <= 256 && parts * 2 <= n_pieces) parts *= 2;
     const int per = 256 / parts;  // items at once
     const int my_part = tid / per;
-    for (int i0 = 0; i0 < n_items; i0 += per) {
+    for (int i0 = (int)blockIdx.z * per; i0 < n_items; i0 += (int)gridDim.z * per) {
         const int i = i0 + tid % per;
         const bool mine = i < n_items;
         const int r = mine ? i % nr : 0, c = mine ? i / nr : 0;  // row; float4 c: 8-group c / 2, half c & 1
@@ -1119,7 +1119,11 @@ hipError_t pa_launch_stream(PagedAttnLaunch p, int ranges, int least, hipStream_
     paged_attn_kernel<DT, T, SRC, true><<<dim3((unsigned)ranges), T::NT, 0, st>>>(p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    paged_combine_kernel<T><<<dim3((unsigned)(ranges - 1), T::RW), 256, 0, st>>>(p, ranges);
+    // few blocks have many pieces each: their elements are shared among more workgroups (64 rows of 8 / 4
+    // heads after 4000 keys, d256: 113 -> 40 us); many blocks: each one more costs a look at the stream
+    const int64_t blocks = pa_max_blocks<T>(p) * p.n_kv_heads;
+    const unsigned share = (unsigned)std::min<int64_t>(std::max<int64_t>(1024 / (blocks * T::RW), 1), T::D / 32);
+    paged_combine_kernel<T><<<dim3((unsigned)(ranges - 1), T::RW, share), 256, 0, st>>>(p, ranges);
     return hipGetLastError();
 }
 
