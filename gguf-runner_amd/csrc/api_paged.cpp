@@ -138,7 +138,9 @@ int check_qo(const char* fn, const void* q, const void* out, int head_dim, int64
     return GR_OK;
 }
 
-int check_fits(const char* fn, const PagedAttnLaunch& p) {
+int check_fits(const char* fn, PagedAttnLaunch& p) {
+    p.group = p.n_heads / p.n_kv_heads;
+    p.group_magic = p.group == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + p.group - 1) / p.group);
     if (!paged_attn_fits(p))
         return fail(GR_ERR_ARG, "%s: rows, sequences and positions beyond 2^31 tiles of work: divide the batch", fn);
     return GR_OK;

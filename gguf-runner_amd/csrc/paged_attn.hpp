@@ -186,13 +186,13 @@ template <int BM, int BN>
 __device__ __forceinline__ PaSeq pa_seq(const PagedAttnLaunch& p, int s) {
     PaSeq r{0, 0, 0, 0, 0};
     if (s >= p.seqs.n_seq) return r;
-    const int group = p.n_heads / p.n_kv_heads;
+    const int group = p.group;
     r.beg = seq_row(p.seqs, s);
     r.n = max(seq_row(p.seqs, s + 1) - r.beg, 0);
     r.len = seq_len(p.seqs, s, r.n);
     r.nb = (r.n * group + BM - 1) / BM;
     r.vt = (r.len + BN - 1) / BN;
-    if (p.window > 0) r.vt = min(r.vt, (min(p.window, r.len) + BM / group + BN - 1) / BN + 1);
+    if (p.window > 0) r.vt = min(r.vt, (min(p.window, r.len) + div_group(p, BM) + BN - 1) / BN + 1);
     r.vt = max(r.vt, 1);
     return r;
 }
@@ -221,8 +221,8 @@ struct PaBlock {
 };
 template <int BM, int BN>
 __device__ __forceinline__ void pa_keys(const PagedAttnLaunch& p, PaBlock& b) {
-    const int group = p.n_heads / p.n_kv_heads;
-    const int tok0 = b.rb * BM / group, tok1 = (min((b.rb + 1) * BM, b.n * group) - 1) / group;
+    const int group = p.group;
+    const int tok0 = div_group(p, b.rb * BM), tok1 = div_group(p, min((b.rb + 1) * BM, b.n * group) - 1);
     b.kend = max(b.p0 + tok1 + 1, 0);
     const int lo = p.window > 0 ? max(b.p0 + tok0 + 1 - p.window, 0) : 0;
     b.all_lo = p.window > 0 ? max(b.p0 + tok1 + 1 - p.window, 0) : 0;
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = KH > 1 ? wave % RW : wave, kh = KH > 1 ? wave / RW : 0;
     const int ln = lane & 31, lg = lane >> 5;
-    const int group = p.n_heads / p.n_kv_heads;
+    const int group = p.group;
     const int shift = p.seqs.page_shift;
     const int ps1 = (1 << shift) - 1;
 
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         const int wr0 = blk.rb * BM + rw * 32;
         const bool wave_active = wr0 < n_pr;
         // the lane's row, its token and position
-        auto token_of = [&](int r) { return min(r, n_pr - 1) / group; };
+        auto token_of = [&](int r) { return div_group(p, min(r, n_pr - 1)); };
         const int my_tok = token_of(wr0 + ln);
         const int my_pos = blk.p0 + my_tok;
         const int my_lo = p.window > 0 ? max(my_pos + 1 - p.window, 0) : 0;
@@ -974,7 +974,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                 continue;
             }
         }
-        const float inv = lsum != 0.0f ? 1.0f / lsum : 0.0f;
+        const float inv = lsum != 0.0f ? __builtin_amdgcn_rcpf(lsum) : 0.0f;  // within an ulp: nothing beside 16 bits
         uint16_t* orow = (uint16_t*)p.out + (int64_t)(blk.beg + tok) * p.out_row_stride +
                          (int64_t)(blk.g * group + (row - tok * group)) * p.out_head_stride;
         const bool f16 = kQ8 ? p.dtype == GR_DTYPE_F16 : std::is_same_v<DT, F16>;
@@ -1009,7 +1009,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunc
     PaBlock blk;
     const int at = pa_stream_find<BM, BN>(p, c0, (w0 + 1) * q, blk);
     if (at == 0 || at > q) return;  // no cut here, or an earlier boundary was in this block
-    const int group = p.n_heads / p.n_kv_heads;
+    const int group = p.group;
     const int r0 = blk.rb * BM + (int)blockIdx.y * 32;
     const int nr = min(32, blk.n * group - r0);
     if (nr <= 0) return;
@@ -1077,7 +1077,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunc
         }
         if (!mine) continue;
         const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        const int tok = (r0 + r) / group, h = blk.g * group + (r0 + r) % group;
+        const int tok = div_group(p, r0 + r), h = blk.g * group + (r0 + r - tok * group);
         uint16_t* out = (uint16_t*)p.out + (int64_t)(blk.beg + tok) * p.out_row_stride + (int64_t)h * p.out_head_stride + 4 * c;
         uint2 y;
         if (p.dtype == GR_DTYPE_F16)
@@ -1093,7 +1093,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunc
 // Blocks of a KV head in a launch at most: every sequence's last block may be partly filled.
 template <typename T>
 int64_t pa_max_blocks(const PagedAttnLaunch& p) {
-    const int64_t rows = (int64_t)p.seqs.n_rows * (p.n_heads / p.n_kv_heads);
+    const int64_t rows = (int64_t)p.seqs.n_rows * p.group;
     return rows / T::BM + std::min<int64_t>(p.seqs.n_seq, p.seqs.n_rows);
 }
 // Places of the stream at most.
@@ -1158,7 +1158,7 @@ struct PaKernels {
     // whole rounds of workgroups where all blocks are about as long and one does not hold them; cut, as its places
     // (each block counts its sequence's longest) and the join.
     static Kind kind(const PagedAttnLaunch& p) {
-        const int group = p.n_heads / p.n_kv_heads;
+        const int group = p.group;
         if (std::min<int64_t>(p.max_rows, p.seqs.n_rows) * group <= Few::BM) return kFew;
         const double len = std::min(p.max_len, p.seqs.max_len), rows = std::min<double>(p.max_rows, len);
         const bool even = p.window > 0 ? len > 2.0 * p.window : rows < 0.4 * len;

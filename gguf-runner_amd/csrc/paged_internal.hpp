@@ -40,6 +40,8 @@ hipError_t launch_paged_kv_read(const PagedKvLaunch& p, hipStream_t st);
 struct PagedAttnLaunch {
     PagedSeqs seqs;
     int n_heads, n_kv_heads, head_dim;
+    int group;             // query heads per KV head
+    uint32_t group_magic;  // ceil(2^32 / group), 0 for 1
     int dtype;     // q, out
     int kv_dtype;  // pages (packed: dtype)
     int window;
@@ -64,6 +66,13 @@ size_t paged_attn_ws_bytes(const PagedAttnLaunch& p);
 hipError_t launch_paged_attn(const PagedAttnLaunch& p, hipStream_t st);
 
 // ---------------------------------------------------------------- device helpers
+
+// r / group for 0 <= r < 2^31: the product with ceil(2^32 / group) is at most one too high.
+__device__ __forceinline__ int div_group(const PagedAttnLaunch& p, int r) {
+    if (p.group == 1) return r;
+    const int q = (int)__umulhi((uint32_t)r, p.group_magic);
+    return q - ((uint32_t)q * (uint32_t)p.group > (uint32_t)r ? 1 : 0);
+}
 
 // Row offset i of the batch, clamped to the row arrays.
 __device__ __forceinline__ int seq_row(const PagedSeqs& s, int i) {
