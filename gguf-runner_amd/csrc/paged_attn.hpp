@@ -82,6 +82,18 @@ struct PaMat<BF16> {
 enum PaMode { kPaFull, kPaMasked, kPaEither };
 enum PaSrc { kPaPacked = 0, kPaPages = 1, kPaPagesQ8 = 2 };
 
+// The launch's arguments (its kernel's only parameter), read anew from here on: what a block uses
+// before or after its tiles does not stay in scalar registers through them.
+__device__ __forceinline__ const PagedAttnLaunch& pa_again() {
+#if defined(__HIP_DEVICE_COMPILE__)
+    auto at = (const __attribute__((address_space(4))) PagedAttnLaunch*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    return *(const PagedAttnLaunch*)at;
+#else
+    return *(const PagedAttnLaunch*)nullptr;
+#endif
+}
+
 // Tiles of a kernel: RW row groups x KH key parts, BN keys, NBUF tiles in LDS (NBUF - 1 of
 // them on their way), waves per SIMD it is built for.
 template <int D_, int RW_, int KH_, int BN_, int NBUF_, int OCC_>
@@ -362,7 +374,6 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = KH > 1 ? wave % RW : wave, kh = KH > 1 ? wave / RW : 0;
     const int ln = lane & 31, lg = lane >> 5;
-    const int group = p.group;
     const int shift = p.seqs.page_shift;
     const int ps1 = (1 << shift) - 1;
 
@@ -413,6 +424,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     }
 
     while (pos < stop) {
+        const PagedAttnLaunch& p = pa_again();
         PaBlock blk;
         int it0 = 0, it1 = 0;
         bool whole = true;
@@ -445,12 +457,11 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             it1 = blk.n_tiles;
         }
 
-        const int n_pr = blk.n * group;
+        const int n_pr = blk.n * p.group;
         const int wr0 = blk.rb * BM + rw * 32;
         const bool wave_active = wr0 < n_pr;
         // the lane's row, its token and position
-        auto token_of = [&](int r) { return div_group(p, min(r, n_pr - 1)); };
-        const int my_tok = token_of(wr0 + ln);
+        const int my_tok = div_group(p, min(wr0 + ln, n_pr - 1));
         const int my_pos = blk.p0 + my_tok;
         const int my_lo = p.window > 0 ? max(my_pos + 1 - p.window, 0) : 0;
         const unsigned my_seen = (unsigned)max(my_pos + 1 - my_lo, 0);
@@ -461,62 +472,84 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         const int lo_max = __builtin_amdgcn_readlane(my_lo, 31);
 
         const int last = blk.kend - 1;
-        const char* const kb0 = (const char*)p.k + (int64_t)blk.g * p.head_stride * EB;
-        const char* const vb0 = (const char*)p.v + (int64_t)blk.g * p.head_stride * EB;
+        const char* kb0 = (const char*)p.k + (int64_t)blk.g * p.head_stride * EB;
+        const char* vb0 = (const char*)p.v + (int64_t)blk.g * p.head_stride * EB;
+        int64_t page_bytes = p.page_stride * EB, row_bytes = p.row_stride * EB;
+        if constexpr (T::OCC == 1 && SRC != kPaPacked) asm volatile("" : "+v"(kb0), "+v"(vb0), "+v"(page_bytes), "+v"(row_bytes));
         int page0 = 0;        // the page Ids[0] is of
         bool some_bad = false, ever_bad = false;  // in the run, in a run so far
 
-        // Page ids of a tile: lane u < LD the page of this wave's rows of round u, lane 32 + j
-        // that of keys 16 j .. 16 j + 15.
-        auto tile_ids = [&](int t0) __attribute__((always_inline)) {
-            if constexpr (SRC == kPaPacked) return 0;
-            const int key = t0 + (lane < 32 ? wave * RPV + min(lane, LD - 1) * RPU : min(lane - 32, BN / 16 - 1) * 16);
-            return Ids[(min(key, last) >> shift) - page0];
+        // Pages: lane u has where in K and V this wave's run of rows of round u is.  One product in
+        // vector registers for all rounds: a scalar one for every round, and every round's place in
+        // LDS kept in scalar registers through the loop, spilled them, and the scheduler gave up the LDS
+        // reads ahead of their products that a single wave per SIMD lives on (head_dim 256, 8000-token
+        // prompt of 8 / 4 heads: 416 -> 312 us).
+        struct Runs {
+            uint64_t k, v;
+        };
+        auto tile_runs = [&](int t0) __attribute__((always_inline)) {
+            if constexpr (SRC == kPaPacked) {
+                return Runs{};
+            } else {
+                const int key = min(t0 + wave * RPV + min(lane, LD - 1) * RPU, last);
+                const int id = max(Ids[(key >> shift) - page0], 0);
+                const int64_t at = (int64_t)id * page_bytes + (int64_t)(key & ps1) * row_bytes;
+                return Runs{(uint64_t)(kb0 + at), (uint64_t)(vb0 + at)};
+            }
+        };
+        auto lane_at = [&](uint64_t x, int u) __attribute__((always_inline)) {
+            return (const char*)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), u) << 32 |
+                                 (uint32_t)__builtin_amdgcn_readlane((int)x, u));
+        };
+        auto round_wave = [&]() __attribute__((always_inline)) {
+            int w = wave;
+            if constexpr (T::OCC == 1) asm volatile("" : "+s"(w));
+            return w;
+        };
+        // Round u's run in K and V (scalar) and the lane's offset in it: rows past the last key repeat it
+        // (they are masked, and must not be read).
+        auto round_of = [&](int t0, const Runs& runs, int w, int u, const char*& k, const char*& v) __attribute__((always_inline)) {
+            const int fc = min(t0 + w * RPV + u * RPU, last);
+            if constexpr (SRC == kPaPacked) {
+                const int64_t at = (int64_t)(blk.beg + fc) * row_bytes;
+                k = kb0 + at;
+                v = vb0 + at;
+            } else {
+                k = lane_at(runs.k, u);
+                v = lane_at(runs.v, u);
+            }
+            return (t0 + BN - 1 <= last ? lrow : min(lrow, last - fc)) * rsb + col(u);
         };
         // 16-key runs of the tile whose page is not there
         auto bad_runs = [&](int t0) __attribute__((always_inline)) {
             if (SRC == kPaPacked || !some_bad) return 0u;
-            return (unsigned)(__ballot(tile_ids(t0) < 0) >> 32) & ((1u << (BN / 16)) - 1);
-        };
-        // For round u of the tile at t0: the byte offset of this wave's run of rows (scalar), and
-        // how far the lane's row may go in it (rows past the last key repeat it: they are
-        // masked, and must not be read).
-        auto run_of = [&](int t0, int ids, int u, int& room) __attribute__((always_inline)) {
-            const int fc = min(t0 + wave * RPV + u * RPU, last);
-            room = last - fc;
-            if constexpr (SRC == kPaPacked) {
-                return (int64_t)(blk.beg + fc) * p.row_stride * EB;
-            } else {
-                const int id = max(__builtin_amdgcn_readlane(ids, u), 0);
-                return ((int64_t)id * p.page_stride + (int64_t)(fc & ps1) * p.row_stride) * EB;
-            }
+            const int key = min(t0 + min(lane, BN / 16 - 1) * 16, last);
+            return (unsigned)__ballot(Ids[(key >> shift) - page0] < 0) & ((1u << (BN / 16)) - 1);
         };
         auto dma_tile = [&](int t0, uint16_t* kd, uint16_t* vd) __attribute__((always_inline)) {
-            const int ids = tile_ids(t0);
-            const bool full = t0 + BN - 1 <= last;
+            const Runs runs = tile_runs(t0);
+            const int w = round_wave();
 #pragma unroll
             for (int u = 0; u < LD; u++) {
-                int room;
-                const int64_t at = run_of(t0, ids, u, room);
-                const int off = (full ? lrow : min(lrow, room)) * rsb + col(u);
-                const int dst = (wave * 64 + u * NT) * 8;
-                pa_dma16(pa_rsrc(kb0 + at), kd + dst, off);
-                pa_dma16(pa_rsrc(vb0 + at), vd + dst, off);
+                const char *k, *v;
+                const int off = round_of(t0, runs, w, u, k, v);
+                const int dst = (w * 64 + u * NT) * 8;
+                pa_dma16(pa_rsrc(k), kd + dst, off);
+                pa_dma16(pa_rsrc(v), vd + dst, off);
             }
         };
         uint4 kr[kQ8 ? LD : 1], vr[kQ8 ? LD : 1];
         float ks_r = 0.0f, vs_r = 1.0f;
         auto load_q8 = [&](int t0) __attribute__((always_inline)) {
             if constexpr (kQ8) {
-                const int ids = tile_ids(t0);
-                const bool full = t0 + BN - 1 <= last;
+                const Runs runs = tile_runs(t0);
+                const int w = round_wave();
 #pragma unroll
                 for (int u = 0; u < LD; u++) {
-                    int room;
-                    const int64_t at = run_of(t0, ids, u, room);
-                    const int off = (full ? lrow : min(lrow, room)) * rsb + col(u);
-                    kr[u] = pa_load16(pa_rsrc(kb0 + at), off);
-                    vr[u] = pa_load16(pa_rsrc(vb0 + at), off);
+                    const char *k, *v;
+                    const int off = round_of(t0, runs, w, u, k, v);
+                    kr[u] = pa_load16(pa_rsrc(k), off);
+                    vr[u] = pa_load16(pa_rsrc(v), off);
                 }
                 if (tid < BN) {
                     const int key = min(t0 + tid, last);
@@ -553,7 +586,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         uint4 qf[D / 16];
         float q_mul = 1.0f;  // Q8: what the scores are multiplied by (bf16 rows are put in f16's range)
         {
-            const int h = blk.g * group + (min(wr0 + ln, n_pr - 1) - my_tok * group);
+            const int h = blk.g * p.group + (min(wr0 + ln, n_pr - 1) - my_tok * p.group);
             const uint16_t* qr = (const uint16_t*)p.q + (int64_t)(blk.beg + my_tok) * p.q_row_stride +
                                  (int64_t)h * p.q_head_stride;
 #pragma unroll
@@ -568,7 +601,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         };
         auto prepare_q = [&]() __attribute__((always_inline)) {
             if constexpr (kQ8) {
-                if (p.dtype == GR_DTYPE_BF16) {
+                if (pa_again().dtype == GR_DTYPE_BF16) {
                     // bf16's 8 significant bits fit f16's 11: exact but for values 2^-24 below the row's largest
                     float big = 0.0f;
 #pragma unroll
@@ -775,6 +808,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             const int n_tiles = min(it1 - rt, run_tiles);
             __syncthreads();  // what ran before is done with every LDS array
             if constexpr (SRC != kPaPacked) {
+                const PagedAttnLaunch& p = pa_again();
                 const int32_t* table = p.seqs.page_table + (int64_t)blk.seq * p.seqs.table_stride;
                 page0 = t_begin >> shift;
                 const int n_ids = (min(last, t_begin + n_tiles * BN - 1) >> shift) - page0 + 1;
@@ -870,6 +904,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         // V elements that are not finite, left out of the partly hidden tiles, a key at a time: p * inf is
         // inf of that sign for every row that sees the key, two signs or a NaN make NaN.  With key
         // parts, part k takes its keys of every tile.
+        const PagedAttnLaunch& pe = pa_again();
         if (!kQ8 && odd) {
 #pragma unroll 1
             for (int it = it0; it < it1; it++) {
@@ -881,11 +916,11 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     if (key > last) break;
                     int64_t at;
                     if constexpr (SRC == kPaPacked) {
-                        at = (int64_t)(blk.beg + key) * p.row_stride;
+                        at = (int64_t)(blk.beg + key) * pe.row_stride;
                     } else {
-                        const int id = p.seqs.page_table[(int64_t)blk.seq * p.seqs.table_stride + (key >> shift)];
-                        if ((unsigned)id >= (unsigned)p.seqs.n_pages) continue;
-                        at = (int64_t)id * p.page_stride + (int64_t)(key & ps1) * p.row_stride;
+                        const int id = pe.seqs.page_table[(int64_t)blk.seq * pe.seqs.table_stride + (key >> shift)];
+                        if ((unsigned)id >= (unsigned)pe.seqs.n_pages) continue;
+                        at = (int64_t)id * pe.page_stride + (int64_t)(key & ps1) * pe.row_stride;
                     }
                     const uint16_t* v = (const uint16_t*)vb0 + at + 4 * lg;
                     if ((unsigned)(key - my_lo) < my_seen) {
@@ -908,7 +943,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         asm volatile("" : "+v"(ln2));
         const int row = wr0 + ln2;
         const bool row_ok = row < n_pr;
-        const int tok = token_of(row);
+        const int tok = div_group(pe, min(row, n_pr - 1));
         if constexpr (KH > 1) {
             // Every key part leaves (O, m, l) of its rows in the tile buffers; part k then adds up its
             // 1 / KH of the row group's O: O = sum O_k 2^(m_k - m), m = max m_k.
@@ -961,7 +996,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         const int first4 = KH > 1 ? kh * N4 : 0;  // ... from this one on
         if constexpr (STREAM) {
             if (!whole) {
-                float* const ws = (float*)p.workspace + (int64_t)(slot * RW + rw) * (32 * D + 64);
+                float* const ws = (float*)pe.workspace + (int64_t)(slot * RW + rw) * (32 * D + 64);
 #pragma unroll
                 for (int i = 0; i < N4; i++)
                     *(float4*)(ws + ((first4 + i) * 64 + lane) * 4) =
@@ -975,9 +1010,9 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
             }
         }
         const float inv = lsum != 0.0f ? __builtin_amdgcn_rcpf(lsum) : 0.0f;  // within an ulp: nothing beside 16 bits
-        uint16_t* orow = (uint16_t*)p.out + (int64_t)(blk.beg + tok) * p.out_row_stride +
-                         (int64_t)(blk.g * group + (row - tok * group)) * p.out_head_stride;
-        const bool f16 = kQ8 ? p.dtype == GR_DTYPE_F16 : std::is_same_v<DT, F16>;
+        uint16_t* orow = (uint16_t*)pe.out + (int64_t)(blk.beg + tok) * pe.out_row_stride +
+                         (int64_t)(blk.g * pe.group + (row - tok * pe.group)) * pe.out_head_stride;
+        const bool f16 = kQ8 ? pe.dtype == GR_DTYPE_F16 : std::is_same_v<DT, F16>;
 #pragma unroll
         for (int i = 0; i < N4; i++) {
             float x[4];
