@@ -16,6 +16,7 @@ namespace {
 
 constexpr int64_t kMaxRowStride = (int64_t)1 << 22;  // a tile's byte offsets stay in 31 bits
 constexpr int64_t kMaxPositions = (int64_t)1 << 30;  // positions plus a tile stay in 31 bits
+constexpr int kMaxKvRows = 1 << 26;  // rows of a write or read: its threads are numbered in 32 bits
 
 bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
 int elem_bytes(int dtype) { return dtype == GR_DTYPE_F32 ? 4 : dtype == GR_DTYPE_Q8 ? 1 : 2; }
@@ -91,6 +92,7 @@ int kv_call(const char* fn, const gr_paged_cache* c, const gr_paged_batch* b, co
     if (!rc) rc = check_batch(fn, c, b, &none);
     if (rc || none) return rc;
     if (!r) return fail(GR_ERR_ARG, "%s: null rows", fn);
+    if (b->n_rows > kMaxKvRows) return fail(GR_ERR_ARG, "%s: n_rows %d above 2^26: divide the batch", fn, b->n_rows);
     if (r->dtype != GR_DTYPE_F32 && r->dtype != GR_DTYPE_F16 && r->dtype != GR_DTYPE_BF16)
         return fail(GR_ERR_ARG, "%s: rows dtype %d unsupported (F32, F16, BF16)", fn, r->dtype);
     if (!r->k || !r->v) return fail(GR_ERR_ARG, "%s: null k or v rows", fn);

@@ -94,8 +94,8 @@ __device__ __forceinline__ const PagedAttnLaunch& pa_again() {
 #endif
 }
 
-// Tiles of a kernel: RW row groups x KH key parts, BN keys, NBUF tiles in LDS (NBUF - 1 of
-// them on their way), waves per SIMD it is built for.
+// Tiles of a kernel: RW row groups x KH key parts, BN keys, NBUF tiles in LDS (with two, one
+// is on its way), waves per SIMD it is built for.
 template <int D_, int RW_, int KH_, int BN_, int NBUF_, int OCC_>
 struct PaTile {
     static constexpr int D = D_, RW = RW_, KH = KH_, BN = BN_, NBUF = NBUF_, OCC = OCC_;
@@ -121,12 +121,8 @@ __device__ __forceinline__ uint4 pa_load16(__amdgpu_buffer_rsrc_t r, int voff) {
     return uint4{};
 #endif
 }
-// s_waitcnt vmcnt(N): all but the last N vector memory operations of the wave are done
-template <int N>
-__device__ __forceinline__ void pa_wait_vmem() {
-    static_assert(N < 64, "vmcnt has 6 bits");
-    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
-}
+// s_waitcnt vmcnt(0): the wave's vector memory operations are done
+__device__ __forceinline__ void pa_wait_vmem() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 __device__ __forceinline__ float pa_xmax32(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -262,7 +258,8 @@ __device__ __forceinline__ int pa_stream_total(const PagedAttnLaunch& p, const P
     }
     return t;
 }
-// The block that place x (< total) belongs to; returns x's offset in it.  c0: pa_seq of the lane.
+// The block that place x (< total) belongs to; returns x's offset in it, -1 for none (only
+// rows that overlap, which sum up to more than 2^31 places).  c0: pa_seq of the lane.
 template <int BM, int BN>
 __device__ __forceinline__ int pa_stream_find(const PagedAttnLaunch& p, const PaSeq& c0, int x, PaBlock& b) {
     for (int s0 = 0; s0 < p.seqs.n_seq; s0 += 64) {
@@ -277,22 +274,21 @@ __device__ __forceinline__ int pa_stream_find(const PagedAttnLaunch& p, const Pa
             const int i = x / b.vt;
             b.g = i / b.nb;
             b.rb = i - b.g * b.nb;
+            if ((unsigned)b.g >= (unsigned)p.n_kv_heads) return -1;
             pa_keys<BM, BN>(p, b);
             return x - i * b.vt;
         }
         x -= all;
     }
-    return 0;
+    return -1;
 }
 
 // Workgroup b of a stream launch as a place among them: XCD b % 8 gets a run of
 // neighbouring ranges (the blocks of a sequence's KV head share its tiles in one L2).
 // Launches are multiples of 8 workgroups.
 __device__ __forceinline__ int pa_stream_rank(int b, int n) { return (b & 7) * (n / 8) + (b >> 3); }
-// Places per range: an equal share, at least least.
-__device__ __forceinline__ int pa_stream_q(int total, int n, int least) {
-    return max((int)(((int64_t)total + n - 1) / n), least);
-}
+// Places per range: an equal share.
+__device__ __forceinline__ int pa_stream_q(int total, int n) { return (int)(((int64_t)total + n - 1) / n); }
 
 // ORDERED: item idx of one KV head, longest blocks first: blocks by their number counted
 // from a sequence's first, the highest numbers first (up to 64 sequences); more sequences:
@@ -350,17 +346,13 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     constexpr int RPV = 64 / SCPR;          // ... of a wave: inside one run of 16 rows, so one page
     constexpr int EB = kQ8 ? 1 : 2;         // bytes per stored element
     static_assert(LD >= 1 && LD <= 32 && BN * SCPR % NT == 0 && BN / 16 <= 32 && BN <= NT, "tile shape");
-    static_assert(kQ8 ? NBUF <= 2 : NBUF == 2 || NBUF == 4, "buffers");
+    static_assert(kQ8 ? NBUF <= 2 : NBUF == 2, "buffers");
 
     // distinct arrays, so that the compiler sees that filling one never aliases reading another
     __shared__ __attribute__((aligned(16))) uint16_t Ks0[BN * D];
     __shared__ __attribute__((aligned(16))) uint16_t Ks1[NBUF > 1 ? BN * D : 8];
     __shared__ __attribute__((aligned(16))) uint16_t Vs0[BN * D];
     __shared__ __attribute__((aligned(16))) uint16_t Vs1[NBUF > 1 ? BN * D : 8];
-    __shared__ __attribute__((aligned(16))) uint16_t Ks2[NBUF == 4 ? BN * D : 8];
-    __shared__ __attribute__((aligned(16))) uint16_t Ks3[NBUF == 4 ? BN * D : 8];
-    __shared__ __attribute__((aligned(16))) uint16_t Vs2[NBUF == 4 ? BN * D : 8];
-    __shared__ __attribute__((aligned(16))) uint16_t Vs3[NBUF == 4 ? BN * D : 8];
     // Q8: c * k_scale, log2 v_scale, 1 / v_scale of the tile's keys
     __shared__ __attribute__((aligned(16))) float Sc0[kQ8 ? 3 * BN : 4];
     __shared__ __attribute__((aligned(16))) float Sc1[kQ8 && NBUF > 1 ? 3 * BN : 4];
@@ -417,7 +409,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
     if constexpr (STREAM) {
         const int total = pa_stream_total<BM, BN>(p, c0);
         rank = pa_stream_rank(blockIdx.x, gridDim.x);
-        const int q = pa_stream_q(total, gridDim.x, p.least);
+        const int q = pa_stream_q(total, gridDim.x);
         if ((int64_t)rank * q >= total) return;
         pos = rank * q;
         stop = min((int64_t)total, (int64_t)pos + q);
@@ -431,6 +423,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         int slot = 0;
         if constexpr (STREAM) {
             const int at = pa_stream_find<BM, BN>(p, c0, pos, blk);
+            if (at < 0) return;
             const int to = min(blk.vt, at + (stop - pos));
             whole = at == 0 && to == blk.vt;
             slot = 2 * rank + (at == 0 ? 1 : 0);
@@ -802,7 +795,7 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
         };
 
         // The tiles, run of page ids by run.
-        const int run_tiles = SRC == kPaPacked ? it1 - it0 : (int)(((int64_t)(kIds - 1) << shift) / BN);
+        const int run_tiles = SRC == kPaPacked ? it1 - it0 : (int)min(((int64_t)(kIds - 1) << shift) / BN, (int64_t)1 << 30);
         for (int rt = it0; rt < it1; rt += run_tiles) {
             const int t_begin = blk.t_first + rt * BN;
             const int n_tiles = min(it1 - rt, run_tiles);
@@ -852,58 +845,30 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                     __syncthreads();
                 }
             } else {
-                auto kbuf = [&](auto i) __attribute__((always_inline)) -> uint16_t* {
-                    constexpr int I = decltype(i)::value % NBUF;
-                    if constexpr (I == 0) return Ks0;
-                    else if constexpr (I == 1) return Ks1;
-                    else if constexpr (I == 2) return Ks2;
-                    else return Ks3;
-                };
-                auto vbuf = [&](auto i) __attribute__((always_inline)) -> uint16_t* {
-                    constexpr int I = decltype(i)::value % NBUF;
-                    if constexpr (I == 0) return Vs0;
-                    else if constexpr (I == 1) return Vs1;
-                    else if constexpr (I == 2) return Vs2;
-                    else return Vs3;
-                };
-                // tile it (buffer I): wait until it is in LDS, send for the tile NBUF - 1 later, compute
-                auto step = [&](auto i, int it) __attribute__((always_inline)) {
-                    constexpr int I = decltype(i)::value;
+                // tile it: wait until it is in LDS, send for the next one, compute
+                auto step = [&](uint16_t* kd, uint16_t* vd, uint16_t* next_kd, uint16_t* next_vd, int it) __attribute__((always_inline)) {
                     const int t0 = t_begin + it * BN;
-                    if (it + NBUF - 2 < n_tiles) pa_wait_vmem<(NBUF - 2) * 2 * LD>();
-                    else pa_wait_vmem<0>();
+                    pa_wait_vmem();
                     __syncthreads();  // everyone's part of it is, and tile it - 1's buffer is free
-                    if (it + NBUF - 1 < n_tiles)
-                        dma_tile(t0 + (NBUF - 1) * BN, kbuf(std::integral_constant<int, I + NBUF - 1>{}),
-                                 vbuf(std::integral_constant<int, I + NBUF - 1>{}));
+                    if (it + 1 < n_tiles) dma_tile(t0 + BN, next_kd, next_vd);
                     const unsigned bad = bad_runs(t0);
-                    if (partly(t0, bad)) finite_only(vbuf(i));
-                    compute_tile(kbuf(i), vbuf(i), Sc0, t0, bad);
+                    if (partly(t0, bad)) finite_only(vd);
+                    compute_tile(kd, vd, Sc0, t0, bad);
                 };
-                using std::integral_constant;
                 dma_tile(t_begin, Ks0, Vs0);
-                if constexpr (NBUF == 4) {
-                    if (n_tiles > 1) dma_tile(t_begin + BN, Ks1, Vs1);
-                    if (n_tiles > 2) dma_tile(t_begin + 2 * BN, Ks2, Vs2);
-                }
                 settle_q();
-                for (int it = 0; it < n_tiles; it += NBUF) {
-                    step(integral_constant<int, 0>{}, it);
+                for (int it = 0; it < n_tiles; it += 2) {
+                    step(Ks0, Vs0, Ks1, Vs1, it);
                     if (it + 1 >= n_tiles) break;
-                    step(integral_constant<int, 1>{}, it + 1);
-                    if constexpr (NBUF == 4) {
-                        if (it + 2 >= n_tiles) break;
-                        step(integral_constant<int, 2>{}, it + 2);
-                        if (it + 3 >= n_tiles) break;
-                        step(integral_constant<int, 3>{}, it + 3);
-                    }
+                    step(Ks1, Vs1, Ks0, Vs0, it + 1);
                 }
             }
         }
 
         // V elements that are not finite, left out of the partly hidden tiles, a key at a time: p * inf is
         // inf of that sign for every row that sees the key, two signs or a NaN make NaN.  With key
-        // parts, part k takes its keys of every tile.
+        // parts, each part takes the keys whose scores it had: its maximum is a number then, and the
+        // merge does not multiply the infinity by 0.
         const PagedAttnLaunch& pe = pa_again();
         if (!kQ8 && odd) {
 #pragma unroll 1
@@ -911,8 +876,8 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
                 const int t0 = blk.t_first + it * BN;
                 if (!partly(t0, SRC == kPaPages && ever_bad)) continue;
 #pragma unroll 1
-                for (int i = kh; i < BN; i += KH) {
-                    const int key = t0 + i;
+                for (int i = 0; i < BN / KH; i++) {
+                    const int key = t0 + 32 * (KH * (i / 32) + kh) + i % 32;
                     if (key > last) break;
                     int64_t at;
                     if constexpr (SRC == kPaPacked) {
@@ -1038,12 +1003,12 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunc
     __shared__ float Sm[256];
     const PaSeq c0 = pa_seq<BM, BN>(p, threadIdx.x & 63);
     const int total = pa_stream_total<BM, BN>(p, c0);
-    const int q = pa_stream_q(total, n_ranges, p.least);
+    const int q = pa_stream_q(total, n_ranges);
     const int w0 = (int)blockIdx.x;  // the range before the boundary
     if ((int64_t)(w0 + 1) * q >= total) return;
     PaBlock blk;
     const int at = pa_stream_find<BM, BN>(p, c0, (w0 + 1) * q, blk);
-    if (at == 0 || at > q) return;  // no cut here, or an earlier boundary was in this block
+    if (at <= 0 || at > q) return;  // no cut here, or an earlier boundary was in this block
     const int group = p.group;
     const int r0 = blk.rb * BM + (int)blockIdx.y * 32;
     const int nr = min(32, blk.n * group - r0);
@@ -1149,8 +1114,7 @@ hipError_t pa_launch_ordered(const PagedAttnLaunch& p, hipStream_t st) {
 }
 
 template <typename DT, typename T, int SRC>
-hipError_t pa_launch_stream(PagedAttnLaunch p, int ranges, int least, hipStream_t st) {
-    p.least = least;
+hipError_t pa_launch_stream(const PagedAttnLaunch& p, int ranges, hipStream_t st) {
     paged_attn_kernel<DT, T, SRC, true><<<dim3((unsigned)ranges), T::NT, 0, st>>>(p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -1229,15 +1193,22 @@ struct PaKernels {
             default: return 256;
         }
     }
+    // Whether a cut call's places can be numbered in 31 bits, an uncut one's threads in 32.
     static bool fits(const PagedAttnLaunch& p) {
-        return std::max({pa_max_places<Few>(p), pa_max_places<FewQ8>(p), pa_max_places<Cut>(p)}) < INT32_MAX;
+        constexpr int64_t kMost = INT32_MAX;
+        switch (kind(p)) {
+            case kFew: return std::max(pa_max_places<Few>(p), pa_max_places<FewQ8>(p)) < kMost;
+            case kCut: return pa_max_places<Cut>(p) < kMost;
+            case kMid: return (pa_max_blocks<Mid>(p) + 8) * p.n_kv_heads * Mid::NT < 2 * kMost;
+            default: return (pa_max_blocks<Big>(p) + 8) * p.n_kv_heads * Big::NT < 2 * kMost;
+        }
     }
     template <typename DT, int SRC>
     static hipError_t launch(const PagedAttnLaunch& p, hipStream_t st) {
         using F = std::conditional_t<SRC == kPaPagesQ8, FewQ8, Few>;
         switch (kind(p)) {
-            case kFew: return pa_launch_stream<DT, F, SRC>(p, n_ranges<F>(p), 1, st);
-            case kCut: return pa_launch_stream<DT, Cut, SRC>(p, n_ranges<Cut>(p), 1, st);
+            case kFew: return pa_launch_stream<DT, F, SRC>(p, n_ranges<F>(p), st);
+            case kCut: return pa_launch_stream<DT, Cut, SRC>(p, n_ranges<Cut>(p), st);
             case kMid: return pa_launch_ordered<DT, Mid, SRC>(p, st);
             default: return pa_launch_ordered<DT, Big, SRC>(p, st);
         }

@@ -56,11 +56,10 @@ struct PagedAttnLaunch {
     const float* v_scale;
     int64_t scale_page_stride, scale_row_stride, scale_head_stride;
     int max_rows, max_len;  // the caller's bounds, for the choice of kernels
-    int least;              // stream launches: places per range at least
     void* workspace;
 };
 
-// Whether the tiles of every call of these bounds can be numbered in 31 bits.
+// Whether the launch's work can be numbered.
 bool paged_attn_fits(const PagedAttnLaunch& p);
 size_t paged_attn_ws_bytes(const PagedAttnLaunch& p);
 hipError_t launch_paged_attn(const PagedAttnLaunch& p, hipStream_t st);

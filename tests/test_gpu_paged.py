@@ -547,3 +547,102 @@ def test_offsets_out_of_range_are_clamped(pkg):
     absent = torch.arange(48) >= 32
     want, bound = ref.attention(q[4:].double(), k, v, 44, 0, 1 / math.sqrt(128), absent)
     check(out[4:], want, bound(F16))
+
+
+# bounds that lead to each of a head_dim's kernels whatever the batch is (they "choose kernels;
+# a wrong value costs time, not results"): few rows, whole blocks, blocks cut along the keys
+HINTS = [(1, 1), (500, 1), (300, 1 << 20), (4096, 1 << 20)]
+
+
+def hinted(ops, b, hint):
+    return ops.PagedBatch(torch.from_numpy(b.start).cuda(), torch.tensor(b.lens, dtype=torch.int32).cuda(),
+                          torch.from_numpy(b.table).cuda(), n_rows=b.n_rows, max_rows=hint[0], max_len=hint[1])
+
+
+@pytest.mark.parametrize("hint", HINTS)
+@pytest.mark.parametrize("h,g,d", [(14, 2, 64), (16, 8, 128), (8, 4, 256)])
+@pytest.mark.parametrize("dtype,kv", [(F16, F16), (BF16, BF16), (F16, Q8), (BF16, Q8)])
+@pytest.mark.parametrize("many,window", [(False, 0), (False, 70), (True, 0)])
+def test_bounds_choose_kernels_not_results(pkg, hint, h, g, d, dtype, kv, many, window):
+    """Every kernel of a head_dim and type over one mixed batch, and over more sequences than a
+    wave has lanes."""
+    from gguf_runner_amd import ops
+    if many:
+        b = ref.Batch([3, 17, 0, 1, 40] * 20, [i % 90 + 40 for i in range(100)], 16, 21, tail=2, table_extra=2000)
+    else:
+        b = ref.Batch([7, 1, 0, 130, 33, 300], [300, 1, 90, 130, 20, 1000], 16, 22, lead=1, tail=3, table_extra=2000)
+    gen = torch.Generator().manual_seed(13)
+    pool = pool_of(gen, b, g, d, kv)
+    q = torch.randn((b.n_rows, h, d), generator=gen).to(dtype)
+    out = torch.full((b.n_rows, h, d), 7.0, dtype=dtype).cuda()
+    before = out.clone()
+    ops.PagedAttentionCall(ops.PagedCache(*pool), hinted(ops, b, hint), q.cuda(), out, window=window)()
+    torch.cuda.synchronize()
+    check_attention(b, out, q, pool, window, 1 / math.sqrt(d), dtype, before)
+
+
+@pytest.mark.parametrize("hint", HINTS)
+@pytest.mark.parametrize("h,g,d", [(14, 2, 64), (16, 8, 128), (8, 4, 256)])
+@pytest.mark.parametrize("kv", [F16, BF16])
+@pytest.mark.parametrize("window", [0, 40])
+def test_infinities_reach_only_the_rows_that_see_them(pkg, hint, h, g, d, kv, window):
+    """Infinite V elements of visible keys, NaN and inf everywhere no sequence has a row, in
+    every kernel of a head_dim."""
+    from gguf_runner_amd import ops
+    b = ref.Batch([1, 90, 200, 5], [100, 90, 250, 37], 16, 23, table_extra=2000)
+    gen = torch.Generator().manual_seed(14)
+    pool = pool_of(gen, b, g, d, kv)
+    marks = {0: [(70, g - 1, 3, math.inf)], 2: [(203, 0, 9, math.inf), (230, g - 1, 40, -math.inf), (60, 0, 11, math.inf)]}
+    own = torch.zeros(b.n_pages, b.page, dtype=torch.bool)
+    for s in range(4):
+        own[tuple(torch.from_numpy(x) for x in b.places(s))] = True
+    hole = (~own).nonzero(as_tuple=True)
+    for i in (0, 1):
+        x = pool[i].cpu()
+        x[hole] = torch.tensor([math.inf, math.nan, -math.inf]).repeat(hole[0].numel())[:hole[0].numel()].view(-1, 1, 1).to(x.dtype)
+        for s, at in marks.items() if i == 1 else ():
+            pg, ro = b.places(s)
+            for pos, head, e, value in at:
+                x[int(pg[pos]), int(ro[pos]), head, e] = value
+        pool[i].copy_(x)
+    q = torch.randn((b.n_rows, h, d), generator=gen).to(kv)
+    out = torch.zeros((b.n_rows, h, d), dtype=kv).cuda()
+    ops.PagedAttentionCall(ops.PagedCache(*pool), hinted(ops, b, hint), q.cuda(), out, window=window)()
+    torch.cuda.synchronize()
+    out = out.cpu()
+    for s in range(4):
+        n, lo = b.rows[s], int(b.start[s])
+        k, v = (stored(b, pool[i], None, s) for i in (0, 1))
+        p0 = b.lens[s] - n
+        pos = torch.arange(p0, p0 + n)
+        hit = torch.zeros(n, h, d, dtype=torch.bool)
+        for at, head, e, value in marks.get(s, []):
+            sees = (pos >= at) & ((pos < at + window) if window else True)
+            hit[sees, head * (h // g):(head + 1) * (h // g), e] = True
+            assert (out[lo:lo + n][sees, head * (h // g):(head + 1) * (h // g), e] == value).all()
+            v[at, head, e] = 0.0
+        want, bound = ref.attention(q[lo:lo + n].double(), k, v, p0, window, 1 / math.sqrt(d))
+        check(out[lo:lo + n][~hit], want[~hit], bound(kv)[~hit], f"sequence {s}")
+
+
+@pytest.mark.parametrize("log_page", [20, 28, 29, 30])
+@pytest.mark.parametrize("kv", [F16, Q8])
+@pytest.mark.parametrize("rows", [1, 100])
+def test_pages_of_any_size(pkg, log_page, kv, rows):
+    """One page per sequence, far larger than the rows that are in it (the memory behind them is
+    never touched): pages of up to 2^30 rows."""
+    from gguf_runner_amd import ops
+    b = ref.Batch([rows], [200], 256, 24, spare=0, table_extra=0)
+    gen = torch.Generator().manual_seed(15)
+    pool = pool_of(gen, b, 2, 64, kv)
+    cache, batch = ops.PagedCache(*pool), b.device(ops)
+    cache.desc.page_size = 1 << log_page
+    q = torch.randn((b.n_rows, 14, 64), generator=gen).to(F16)
+    out = torch.full((b.n_rows, 14, 64), 7.0, dtype=F16).cuda()
+    ops.PagedAttentionCall(cache, batch, q.cuda(), out)()
+    back = [torch.empty((b.n_rows, 2, 64), dtype=F32).cuda() for _ in "kv"]
+    ops.PagedReadCall(cache, batch, *back)()
+    torch.cuda.synchronize()
+    check_attention(b, out, q, pool, 0, 1 / 8, F16, out)
+    for i in (0, 1):
+        assert torch.equal(back[i].cpu().double(), stored(b, pool[i], pool[2 + i], 0)[200 - rows:].float().double())

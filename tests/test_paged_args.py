@@ -153,6 +153,13 @@ def test_more_work_than_can_be_numbered(pkg):
     big = dict(n_seq=1 << 20, n_rows=1 << 20, table_pages=1 << 20, table_stride=1 << 20)
     refused(ffi, L.gr_paged_attention(cache(ffi), batch(ffi, **big), attn(ffi), None), "divide the batch")
     assert L.gr_paged_attention_workspace_size(cache(ffi), batch(ffi, **big), attn(ffi)) == 0
+    # the limit is the one of the kernel that the call takes: the places of a stream where blocks
+    # are cut (max_rows 1), the threads of a launch where they are not
+    rows_of = dict(n_seq=1 << 12, n_rows=1 << 21, table_pages=1 << 14, table_stride=1 << 14, max_len=4096)
+    refused(ffi, L.gr_paged_attention(cache(ffi), batch(ffi, max_rows=1, **rows_of), attn(ffi), None), "divide the batch")
+    assert L.gr_paged_attention_workspace_size(cache(ffi), batch(ffi, max_rows=4096, **rows_of), attn(ffi)) == 256
+    for fn in (L.gr_paged_kv_write, L.gr_paged_kv_read):
+        refused(ffi, fn(cache(ffi), batch(ffi, n_rows=(1 << 26) + 1), rows(ffi), None), "divide the batch")
 
 
 def test_null_and_workspace(pkg):
