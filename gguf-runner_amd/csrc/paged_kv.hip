@@ -5,24 +5,49 @@
 // and V.  A row's K (or V) is n_kv_heads * head_dim / 8 pieces of 8 elements, and a wave
 // takes one row (several when a row has fewer than 64 pieces) of K or V, a piece per
 // lane, so both sides move in whole lines.  The wave finds its row's sequence by a
-// 64-ary search of row_start (one load for up to 63 sequences); a row's values are
-// requested before the search so that its latency hides theirs.
+// 64-ary search of row_start (one load for up to 63 sequences), then its page id; a wave whose
+// rows are all of one sequence reads that sequence's sizes once.
+//
+// Calls that fill the GPU (kPagedKvFull) take U = 4 rows per wave, all requested before the
+// first is used: one row leaves too few bytes in flight (Q8 pages of 3 x 20k .. 32k rows read
+// as bf16: 107 us with one, 60 with 4, 71 with 2, 60 with 8), four in a small call leave CUs
+// idle.  They move what no cache will hold, so whole-line stores and the pages that are read
+// carry the nontemporal hint (that read: 59.3 -> 53.8 us = 5.3 TB/s; f16 pages, 4 x 16k rows:
+// 105 -> 91 us; 4 x 8k rows written: 54 -> 52).  Not so the rows of a write, just computed
+// (with it 4 prompts requantised and read back: 36.5 -> 38.4 us), the 8-byte stores of codes,
+// half a line a row (36.5 -> 39.2), and small calls (20 x 300 rows read: 9.2 -> 11.5 us).
+// Steps of a few rows are bound by the launch and three dependent loads (48 rows: 3.6 - 4.2 us).
 #include "gr_common.hpp"
 #include "paged_internal.hpp"
 
 namespace gr {
 
 constexpr int kPagedKvThreads = 256;
-constexpr int kPagedKvFull = 1024;  // workgroups from which on a wave takes more rows
+constexpr int kPagedKvFull = 1024;  // workgroups (four per CU) from which on a wave takes more rows
+
+// 8 or 16 bytes; ONCE: with the nontemporal hint.
+template <typename V>
+using PkVec = uint32_t __attribute__((ext_vector_type(sizeof(V) / 4)));
+template <typename V, bool ONCE>
+__device__ __forceinline__ V pk_load(const void* p) {
+    if constexpr (ONCE) return __builtin_bit_cast(V, __builtin_nontemporal_load((const PkVec<V>*)p));
+    else return *(const V*)p;
+}
+template <bool ONCE, typename V>
+__device__ __forceinline__ void pk_put(void* p, const V& x) {
+    if constexpr (ONCE) __builtin_nontemporal_store(__builtin_bit_cast(PkVec<V>, x), (PkVec<V>*)p);
+    else *(V*)p = x;
+}
 
 // 8 consecutive elements as they are stored: 8 (codes), 16 or 32 bytes.
 template <int BYTES>
 struct PkRaw {
     using V = std::conditional_t<BYTES == 8, uint2, uint4>;
     V w[BYTES == 32 ? 2 : 1];
+    template <bool ONCE>
     __device__ __forceinline__ void load(const void* p) {
-        w[0] = ((const V*)p)[0];
-        if constexpr (BYTES == 32) w[1] = ((const V*)p)[1];
+        w[0] = pk_load<V, ONCE>(p);
+        if constexpr (BYTES == 32) w[1] = pk_load<V, ONCE>((const V*)p + 1);
     }
     template <typename T>
     __device__ __forceinline__ void floats(float* x) const {
@@ -31,17 +56,17 @@ struct PkRaw {
     }
 };
 
-template <typename T>
+template <typename T, bool ONCE>
 __device__ __forceinline__ void pk_store8(typename T::storage* dst, const float* x) {
     if constexpr (T::bytes == 4) {
-        ((float4*)dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        ((float4*)dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        pk_put<ONCE>(dst, make_float4(x[0], x[1], x[2], x[3]));
+        pk_put<ONCE>(dst + 4, make_float4(x[4], x[5], x[6], x[7]));
     } else {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; i++)
             w[i] = (uint32_t)from_f32<T>(x[2 * i]) | ((uint32_t)from_f32<T>(x[2 * i + 1]) << 16);
-        *(uint4*)dst = make_uint4(w[0], w[1], w[2], w[3]);
+        pk_put<ONCE>(dst, make_uint4(w[0], w[1], w[2], w[3]));
     }
 }
 
@@ -85,6 +110,7 @@ template <int D, typename ROWS, typename KV, bool WRITE, int U>
 __global__ __launch_bounds__(kPagedKvThreads) void paged_kv_kernel(const PagedKvLaunch p, const int lanes_per_row) {
     constexpr int CPH = D / 8;  // pieces per head
     constexpr bool q8 = std::is_same_v<KV, KvQ8>;
+    constexpr bool kStoreOnce = U > 1, kLoadOnce = U > 1 && !WRITE;
     using RT = typename ROWS::storage;
     const int lane = threadIdx.x & 63;
     const int unit = (int)blockIdx.x * (kPagedKvThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -134,15 +160,15 @@ __global__ __launch_bounds__(kPagedKvThreads) void paged_kv_kernel(const PagedKv
             const int row = min(first + u * rpw + lane / lanes_per_row, p.seqs.n_rows - 1);
             const int64_t page = max(at[u].page, 0);
             if constexpr (WRITE) {
-                raw[u].load((const RT*)p.rows[which] + (int64_t)row * p.rows_row_stride + g * p.rows_head_stride + i);
+                raw[u].template load<kLoadOnce>((const RT*)p.rows[which] + (int64_t)row * p.rows_row_stride + g * p.rows_head_stride + i);
             } else {
                 const int64_t e = page * p.page_stride + (int64_t)at[u].row * p.row_stride + g * p.head_stride + i;
                 if constexpr (q8) {
-                    raw[u].load((const int8_t*)p.pages[which] + e);
+                    raw[u].template load<kLoadOnce>((const int8_t*)p.pages[which] + e);
                     sc[u] = p.scale[which][page * p.scale_page_stride + (int64_t)at[u].row * p.scale_row_stride +
                                            g * p.scale_head_stride];
                 } else {
-                    raw[u].load((const typename ST::storage*)p.pages[which] + e);
+                    raw[u].template load<kLoadOnce>((const typename ST::storage*)p.pages[which] + e);
                 }
             }
         }
@@ -168,7 +194,7 @@ __global__ __launch_bounds__(kPagedKvThreads) void paged_kv_kernel(const PagedKv
             const int row = first + u * rpw + lane / lanes_per_row;
             if constexpr (!WRITE) {
                 if (at[u].page != -2)
-                    pk_store8<ROWS>((RT*)p.rows[which] + (int64_t)row * p.rows_row_stride + g * p.rows_head_stride + i, x[u]);
+                    pk_store8<ROWS, kStoreOnce>((RT*)p.rows[which] + (int64_t)row * p.rows_row_stride + g * p.rows_head_stride + i, x[u]);
             } else {
                 const int64_t e = (int64_t)at[u].page * p.page_stride + (int64_t)at[u].row * p.row_stride + g * p.head_stride + i;
                 if constexpr (q8) {
@@ -192,7 +218,7 @@ __global__ __launch_bounds__(kPagedKvThreads) void paged_kv_kernel(const PagedKv
                         p.scale[which][(int64_t)at[u].page * p.scale_page_stride + (int64_t)at[u].row * p.scale_row_stride +
                                        g * p.scale_head_stride] = amax == 0.0f ? 1.0f : amax * (1.0f / 127.0f);
                 } else if (at[u].page >= 0) {
-                    pk_store8<KV>((typename KV::storage*)p.pages[which] + e, x[u]);
+                    pk_store8<KV, kStoreOnce>((typename KV::storage*)p.pages[which] + e, x[u]);
                 }
             }
         }
