@@ -23,6 +23,19 @@
 // Two schedules.  ORDERED: one block per workgroup, longest first.  STREAM: the blocks'
 // tiles, one after another, are cut into one equal range per workgroup; a block that a cut
 // divides leaves unnormalised partials (O, m, l) which paged_combine_kernel joins.
+//
+// What bounds the kernels, on one MI355X:
+//   few rows (up to 32 per sequence and KV head): HBM.  16 tokens of 1k .. 32k keys, f16, 32 / 4
+//     heads, head_dim 128: 97 us = 5.5 TB/s; Q8 pages, 24 sequences of 0.3k .. 12k keys, 1 - 5 rows:
+//     101 us = 3.5 TB/s, where turning codes into f16 takes VALU time of the size of the softmax.  One
+//     tile on its way and one wave per SIMD measured better than more of either (129 against 111 us
+//     with four tiles in LDS, 188 against 108 us for Q8 at two waves per SIMD, which spills).
+//   many rows: the matrix units and the softmax between them (VALU).  Three prompts of 1001 .. 8192
+//     rows, f16, 32 / 8 heads, head_dim 128: 1205 - 1230 us = 950 - 970 TFLOP/s; one of 8192 rows, 8 / 4
+//     heads, head_dim 256: 300 us = 900 TFLOP/s (409 us before its LDS reads went four products
+//     ahead of their use); 40 prompts of 9 .. 777 rows, bf16, 14 / 2 heads, head_dim 64: 36 us, a third
+//     of it short blocks' starts and ends.  At head_dim 256 a block's O, Q and S take a whole SIMD's
+//     registers; two waves per SIMD spill (2900 us).
 #pragma once
 
 #include <algorithm>
@@ -1000,8 +1013,10 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
 }
 
 // Joins the pieces of the block that boundary w (the start of range w) is the first to cut;
-// blockIdx.y: a row group of it, blockIdx.z: a share of its rows' elements.  Thread (row, 4 elements) runs over the pieces; with few rows
-// the workgroup's spare threads share a row's pieces among them and add up in LDS.
+// blockIdx.y: a row group of it, blockIdx.z: a share of its rows' elements.  Thread (row, 4
+// elements) runs over the pieces; with few rows the workgroup's spare threads share a row's
+// pieces among them and add up in LDS.  Bound by latency: 4 us after a token's split kernel, 10
+// after that of 501 rows after 7690 keys (256 ranges of 256-row blocks, 33 MB of partials).
 template <typename T>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunch p, const int n_ranges) {
     constexpr int D = T::D, RW = T::RW, BM = T::BM, BN = T::BN;
@@ -1151,9 +1166,12 @@ struct PaTime {
 };
 
 // The kernels of a head_dim and which of them a call takes.  Few: blocks of few rows, key
-// parts (FewQ8 over Q8 pages), always cut; Mid, Big: one block per workgroup (tMid, tBig), or
-// Cut (its t and what cutting costs, joining included): the tiles of all blocks in equal ranges.
-// Costs: kMid, kBig, kCut, kCutFixed.
+// parts (FewQ8 over Q8 pages), always cut; Mid, Big: one block per workgroup (kMid, kBig), or
+// Cut: the tiles of all blocks in equal ranges (kCut: a tile, cutting and joining included;
+// kCutFixed: the launches of it).  Fitted to calls timed all three ways; head_dim 256, us for
+// Mid / Big / Cut: a prompt of 8000 rows 397 / 312 / 548, 512 rows after 2000 keys 68 / 94 / 37,
+// 8 x 500 rows after 3000 keys 178 / 143 / 148, 24 x 64 rows in a window of 1024 49 / 61 / 60,
+// 4000 rows over Q8 pages 148 / 192 / 194: the rule took the least of the three in each.
 template <typename Few, typename FewQ8, typename Mid, typename Big, typename Cut, typename Costs>
 struct PaKernels {
     enum Kind { kFew, kMid, kBig, kCut };
@@ -1162,8 +1180,8 @@ struct PaKernels {
     static constexpr int ranges = kCus * T::kPerCu;
 
     // Uncut, a launch lasts as long as its longest block alone, or as its tiles take on full CUs,
-    // whole rounds of workgroups where all blocks are about as long and one does not hold them; cut, as its places
-    // (each block counts its sequence's longest) and the join.
+    // whole rounds of workgroups where all blocks are about as long and one round does not hold them;
+    // cut, as its places (each block counts its sequence's longest) and the join.
     static Kind kind(const PagedAttnLaunch& p) {
         const int group = p.group;
         if (std::min<int64_t>(p.max_rows, p.seqs.n_rows) * group <= Few::BM) return kFew;

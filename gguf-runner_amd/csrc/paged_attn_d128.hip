@@ -1,4 +1,9 @@
 // head_dim 128 of the attention over pages and packed rows (paged_attn.hpp).
+//
+// Eight waves of 32 rows share a 128-key tile where there are blocks enough (one workgroup per
+// CU, two waves per SIMD: a wave's softmax runs under the other's products), four waves of a
+// 64-key tile where there are not.  Cut calls take the large block: 501 rows after 7690 keys,
+// 32 / 8 heads, f16: 92 us, 124 with the small one, whose blocks leave twice the partials.
 #include "paged_attn.hpp"
 
 namespace gr {

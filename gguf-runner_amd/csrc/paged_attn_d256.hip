@@ -1,4 +1,9 @@
 // head_dim 256 of the attention over pages and packed rows (paged_attn.hpp).
+//
+// A wave's O, Q and S fill a SIMD's registers, so one wave per SIMD: LDS reads are sent ahead of
+// their products by hand (pa_pipeline).  Few rows over Q8 pages: one tile in LDS instead of
+// two, so that two workgroups share a CU and one converts codes while the other multiplies
+// (16 tokens of 30k keys, 8 / 4 heads: 343 -> 199 us; f16 pages come by DMA and keep two).
 #include "paged_attn.hpp"
 
 namespace gr {

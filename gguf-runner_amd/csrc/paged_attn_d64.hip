@@ -1,4 +1,9 @@
 // head_dim 64 of the attention over pages and packed rows (paged_attn.hpp).
+//
+// Short rows make the softmax the larger part of a tile, so several small workgroups share a
+// CU and hide each other's: 128-row blocks, three waves per SIMD (40 prompts of 9 .. 777 rows,
+// bf16, 14 / 2 heads: 35.1 us; four waves 35.2, 64-row blocks 43.6, 256-row blocks 36 - 41).
+// One kernel is both Mid and Big.
 #include "paged_attn.hpp"
 
 namespace gr {
