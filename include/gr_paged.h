@@ -89,7 +89,7 @@ typedef struct gr_paged_rows {
  * 2^-100 counts as 0: scale 1, codes 0.  A NaN stores as 0; an infinity makes its head
  * row read as NaN. A row whose page id names no page is
  * dropped.  Sequences may share pages they only read; no two rows of a call may name
- * the same place. */
+ * the same place.  At most 2^26 rows, as a read. */
 int gr_paged_kv_write(const gr_paged_cache* c, const gr_paged_batch* b, const gr_paged_rows* rows, void* stream);
 
 /* The reverse: the batch's positions read out of their pages into rows (with kv_len
@@ -103,7 +103,8 @@ int gr_paged_kv_read(const gr_paged_cache* c, const gr_paged_batch* b, const gr_
  * h / (n_heads / n_kv_heads).  Scores, softmax and sums are f32; the weights enter the
  * product with V rounded to dtype (f16 over Q8 pages), the result is rounded once.  A
  * row that sees no key (negative position, pages that hold no rows) gets zeros.  Keys a
- * row does not see have no influence on it, whatever they hold (inf and NaN too). */
+ * row does not see have no influence on it, whatever they hold (inf and NaN too).  More
+ * work than can be numbered in 31 bits of tiles is refused. */
 typedef struct gr_paged_attention_args {
     int32_t n_heads;        /* a multiple of the cache's n_kv_heads */
     int32_t dtype;          /* of q and out: GR_DTYPE_F16 or GR_DTYPE_BF16; the pages' type unless they are Q8 */
