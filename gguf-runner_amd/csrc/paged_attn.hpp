@@ -1014,8 +1014,9 @@ __global__ __launch_bounds__(T::NT, T::OCC) void paged_attn_kernel(const PagedAt
 
 // Joins the pieces of the block that boundary w (the start of range w) is the first to cut;
 // blockIdx.y: a row group of it, blockIdx.z: a share of its rows' elements.  Thread (row, 4
-// elements) runs over the pieces; with few rows the workgroup's spare threads share a row's
-// pieces among them and add up in LDS.  Bound by latency: 4 us after a token's split kernel, 10
+// elements) runs over the pieces, four at once; with more than four and threads to spare,
+// several take a row's pieces among them and add up in LDS (a token after 16000 keys, 32 / 4
+// heads d128: 127 pieces a block, 41 -> 24 us a call; after 1000 keys 13.6 -> 12.2).  Bound by latency: 4 us after a token's split kernel, 10
 // after that of 501 rows after 7690 keys (256 ranges of 256-row blocks, 33 MB of partials).
 template <typename T>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunch p, const int n_ranges) {
@@ -1044,8 +1045,10 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunc
     auto piece = [&](int k) { return ws + (int64_t)(2 * (w0 + k) + (k == 0 ? 1 : 0)) * RW * kUnit; };
     const int tid = threadIdx.x;
     const int n_items = nr * (D / 4);
+    const int my_items = (n_items + (int)gridDim.z - 1) / (int)gridDim.z;
     int parts = 1;  // threads per item, a power of two
-    while (n_items * parts * 2 <= 256 && parts * 2 <= n_pieces) parts *= 2;
+    constexpr int U = 4;  // pieces at once
+    while (my_items * parts * 2 <= 256 && parts * U < n_pieces) parts *= 2;
     const int per = 256 / parts;  // items at once
     const int my_part = tid / per;
     for (int i0 = (int)blockIdx.z * per; i0 < n_items; i0 += (int)gridDim.z * per) {
@@ -1056,7 +1059,6 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunc
         float m = kPaNone, l = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         if (mine) {
-            constexpr int U = 4;  // pieces at once
             for (int k0 = my_part; k0 < n_pieces; k0 += U * parts) {
                 float4 v[U];
                 float mk[U], lk[U];
@@ -1083,7 +1085,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedAttnLaunc
                 }
             }
         }
-        if (parts > 1) {  // n_items * parts <= 256: one round
+        if (parts > 1) {  // my_items * parts <= 256: one round
             So[tid] = o, Sl[tid] = l, Sm[tid] = m;
             __syncthreads();
             if (my_part != 0 || !mine) return;
@@ -1142,7 +1144,8 @@ hipError_t pa_launch_stream(const PagedAttnLaunch& p, int ranges, hipStream_t st
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // few blocks have many pieces each: their elements are shared among more workgroups (64 rows of 8 / 4
-    // heads after 4000 keys, d256: 113 -> 40 us); many blocks: each one more costs a look at the stream
+    // heads after 4000 keys, d256: 113 -> 40 us); many blocks: each one more costs a look at the stream (twice as many: 501 rows after 7690
+    // keys, d128, 94.5 -> 97.7 us; up to 16 of a token after 8000 keys, 32 / 4 heads, 19.8 -> 22.3)
     const int64_t blocks = pa_max_blocks<T>(p) * p.n_kv_heads;
     const unsigned share = (unsigned)std::min<int64_t>(std::max<int64_t>(1024 / (blocks * T::RW), 1), T::D / 32);
     paged_combine_kernel<T><<<dim3((unsigned)(ranges - 1), T::RW, share), 256, 0, st>>>(p, ranges);
