@@ -1144,8 +1144,9 @@ hipError_t pa_launch_stream(const PagedAttnLaunch& p, int ranges, hipStream_t st
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // few blocks have many pieces each: their elements are shared among more workgroups (64 rows of 8 / 4
-    // heads after 4000 keys, d256: 113 -> 40 us); many blocks: each one more costs a look at the stream (twice as many: 501 rows after 7690
-    // keys, d128, 94.5 -> 97.7 us; up to 16 of a token after 8000 keys, 32 / 4 heads, 19.8 -> 22.3)
+    // heads after 4000 keys, d256: 113 -> 40 us); many blocks: each one more costs a
+    // look at the stream (twice as many: 501 rows after 7690 keys, d128, 94.5 -> 97.7 us; up to 16 of
+    // a token after 8000 keys, 32 / 4 heads, 19.8 -> 22.3)
     const int64_t blocks = pa_max_blocks<T>(p) * p.n_kv_heads;
     const unsigned share = (unsigned)std::min<int64_t>(std::max<int64_t>(1024 / (blocks * T::RW), 1), T::D / 32);
     paged_combine_kernel<T><<<dim3((unsigned)(ranges - 1), T::RW, share), 256, 0, st>>>(p, ranges);
@@ -1169,15 +1170,16 @@ struct PaTime {
 };
 
 // The kernels of a head_dim and which of them a call takes.  Few: blocks of few rows, key
-// parts (FewQ8 over Q8 pages), always cut; Mid, Big: one block per workgroup (kMid, kBig), or
+// parts (FewQ8 over Q8 pages), always cut; Wide: the same with larger tiles, for few and long
+// blocks, whose pieces are then fewer (Few where a head_dim has none); Mid, Big: one block per workgroup (kMid, kBig), or
 // Cut: the tiles of all blocks in equal ranges (kCut: a tile, cutting and joining included;
 // kCutFixed: the launches of it).  Fitted to calls timed all three ways; head_dim 256, us for
 // Mid / Big / Cut: a prompt of 8000 rows 397 / 312 / 548, 512 rows after 2000 keys 68 / 94 / 37,
 // 8 x 500 rows after 3000 keys 178 / 143 / 148, 24 x 64 rows in a window of 1024 49 / 61 / 60,
 // 4000 rows over Q8 pages 148 / 192 / 194: the rule took the least of the three in each.
-template <typename Few, typename FewQ8, typename Mid, typename Big, typename Cut, typename Costs>
+template <typename Few, typename FewQ8, typename Wide, typename Mid, typename Big, typename Cut, typename Costs>
 struct PaKernels {
-    enum Kind { kFew, kMid, kBig, kCut };
+    enum Kind { kFew, kWide, kMid, kBig, kCut };
     static constexpr int kCus = 256;
     template <typename T>
     static constexpr int ranges = kCus * T::kPerCu;
@@ -1187,8 +1189,15 @@ struct PaKernels {
     // cut, as its places (each block counts its sequence's longest) and the join.
     static Kind kind(const PagedAttnLaunch& p) {
         const int group = p.group;
-        if (std::min<int64_t>(p.max_rows, p.seqs.n_rows) * group <= Few::BM) return kFew;
-        const double len = std::min(p.max_len, p.seqs.max_len), rows = std::min<double>(p.max_rows, len);
+        const double len = std::min(p.max_len, p.seqs.max_len);
+        if (std::min<int64_t>(p.max_rows, p.seqs.n_rows) * group <= Few::BM) {
+            // one block per sequence and KV head; Few / Wide, f16, d128, us: 1 x 16000 keys, 4 KV heads 23.6 /
+            // 18.7, 4 x 4000 20.3 / 16.4, 1 x 4000, 8 KV heads 15.8 / 14.0; but 1 x 1000 12.3 / 12.9, 16 x 1k ..
+            // 32k, 4 KV heads 97 / 98 - 100, and Q8 pages of 24 sequences to 12k keys, 8 KV heads 101 / 112
+            const int64_t n = (int64_t)std::min(p.seqs.n_seq, p.seqs.n_rows) * p.n_kv_heads;
+            return !std::is_same_v<Wide, Few> && n <= kCus / 8 && len >= 16 * Wide::BN ? kWide : kFew;
+        }
+        const double rows = std::min<double>(p.max_rows, len);
         const bool even = p.window > 0 ? len > 2.0 * p.window : rows < 0.4 * len;
         auto blocks = [&](int bm) {  // half of every sequence's last block is empty
             return ((double)p.seqs.n_rows * group / bm + 0.5 * std::min(p.seqs.n_seq, p.seqs.n_rows)) * p.n_kv_heads;
@@ -1218,6 +1227,7 @@ struct PaKernels {
     static size_t ws(const PagedAttnLaunch& p) {
         switch (kind(p)) {
             case kFew: return p.kv_dtype == GR_DTYPE_Q8 ? pa_ws_bytes<FewQ8>(n_ranges<FewQ8>(p)) : pa_ws_bytes<Few>(n_ranges<Few>(p));
+            case kWide: return pa_ws_bytes<Wide>(n_ranges<Wide>(p));
             case kCut: return pa_ws_bytes<Cut>(n_ranges<Cut>(p));
             default: return 256;
         }
@@ -1227,6 +1237,7 @@ struct PaKernels {
         constexpr int64_t kMost = INT32_MAX;
         switch (kind(p)) {
             case kFew: return std::max(pa_max_places<Few>(p), pa_max_places<FewQ8>(p)) < kMost;
+            case kWide: return pa_max_places<Wide>(p) < kMost;
             case kCut: return pa_max_places<Cut>(p) < kMost;
             case kMid: return (pa_max_blocks<Mid>(p) + 8) * p.n_kv_heads * Mid::NT < 2 * kMost;
             default: return (pa_max_blocks<Big>(p) + 8) * p.n_kv_heads * Big::NT < 2 * kMost;
@@ -1237,6 +1248,9 @@ struct PaKernels {
         using F = std::conditional_t<SRC == kPaPagesQ8, FewQ8, Few>;
         switch (kind(p)) {
             case kFew: return pa_launch_stream<DT, F, SRC>(p, n_ranges<F>(p), st);
+            case kWide:
+                if constexpr (!std::is_same_v<Wide, Few>) return pa_launch_stream<DT, Wide, SRC>(p, n_ranges<Wide>(p), st);
+                return hipErrorInvalidValue;
             case kCut: return pa_launch_stream<DT, Cut, SRC>(p, n_ranges<Cut>(p), st);
             case kMid: return pa_launch_ordered<DT, Mid, SRC>(p, st);
             default: return pa_launch_ordered<DT, Big, SRC>(p, st);

@@ -12,7 +12,8 @@ struct Costs128 {
     static constexpr PaTime kMid{1.6f, 1.2f, 5.0f}, kBig{4.0f, 4.4f, 10.0f}, kCut{4.4f, 4.4f, 0.0f};
     static constexpr float kCutFixed = 18.0f;
 };
-using K128 = PaKernels<PaTile<128, 1, 2, 64, 2, 1>, PaTile<128, 1, 2, 64, 2, 1>, PaTile<128, 4, 1, 64, 2, 2>,
+using K128 = PaKernels<PaTile<128, 1, 2, 64, 2, 1>, PaTile<128, 1, 2, 64, 2, 1>,
+                       PaTile<128, 1, 4, 128, 2, 1>, PaTile<128, 4, 1, 64, 2, 2>,
                        PaTile<128, 8, 1, 128, 2, 2>, PaTile<128, 8, 1, 128, 2, 2>, Costs128>;
 
 bool paged_attn_fits_d128(const PagedAttnLaunch& p) { return K128::fits(p); }

@@ -12,7 +12,8 @@ struct Costs256 {
     static constexpr PaTime kMid{2.0f, 1.75f, 11.0f}, kBig{3.05f, 2.6f, 11.0f}, kCut{3.0f, 3.0f, 0.0f};
     static constexpr float kCutFixed = 24.0f;
 };
-using K256 = PaKernels<PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 1, 2, 64, 1, 1>, PaTile<256, 2, 2, 64, 2, 1>,
+using K256 = PaKernels<PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 1, 2, 64, 1, 1>,
+                       PaTile<256, 1, 2, 64, 2, 1>, PaTile<256, 2, 2, 64, 2, 1>,
                        PaTile<256, 4, 1, 64, 2, 1>, PaTile<256, 4, 1, 64, 2, 1>, Costs256>;
 
 bool paged_attn_fits_d256(const PagedAttnLaunch& p) { return K256::fits(p); }

@@ -12,8 +12,9 @@ struct Costs64 {
     static constexpr PaTime kMid{1.0f, 0.74f, 3.0f}, kBig{1.0f, 0.74f, 3.0f}, kCut{2.4f, 2.4f, 0.0f};
     static constexpr float kCutFixed = 18.0f;
 };
-using K64 = PaKernels<PaTile<64, 1, 4, 128, 2, 2>, PaTile<64, 1, 4, 128, 2, 2>, PaTile<64, 4, 1, 64, 2, 3>, PaTile<64, 4, 1, 64, 2, 3>,
-                      PaTile<64, 8, 1, 128, 2, 2>, Costs64>;
+using K64 = PaKernels<PaTile<64, 1, 4, 128, 2, 2>, PaTile<64, 1, 4, 128, 2, 2>,
+                      PaTile<64, 1, 4, 128, 2, 2>, PaTile<64, 4, 1, 64, 2, 3>,
+                      PaTile<64, 4, 1, 64, 2, 3>, PaTile<64, 8, 1, 128, 2, 2>, Costs64>;
 
 bool paged_attn_fits_d64(const PagedAttnLaunch& p) { return K64::fits(p); }
 size_t paged_attn_ws_d64(const PagedAttnLaunch& p) { return K64::ws(p); }

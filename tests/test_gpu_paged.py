@@ -103,7 +103,7 @@ def test_window_over_pages(pkg, h, g, d, window, dtype, kv):
     run_attention(pkg, b, h, g, d, dtype, kv, window=window)
 
 
-@pytest.mark.parametrize("rows,lens", [([1], [5003]), ([1, 1, 1], [4100, 31, 2500]), ([5] * 3, [3001, 6, 1700]),
+@pytest.mark.parametrize("rows,lens", [([1], [5003]), ([1], [70001]), ([1, 1, 1], [4100, 31, 2500]), ([5] * 3, [3001, 6, 1700]),
                                        ([61], [2900]), ([300], [1903]), ([1] * 70, list(range(1, 71)))])
 @pytest.mark.parametrize("dtype,kv,h,g,d", [(F16, F16, 32, 8, 128), (BF16, BF16, 8, 4, 256), (F16, Q8, 32, 8, 128),
                                             (BF16, Q8, 14, 2, 64), (F16, Q8, 8, 4, 256)])
@@ -551,7 +551,7 @@ def test_offsets_out_of_range_are_clamped(pkg):
 
 # bounds that lead to each of a head_dim's kernels whatever the batch is (they "choose kernels;
 # a wrong value costs time, not results"): few rows, whole blocks, blocks cut along the keys
-HINTS = [(1, 1), (500, 1), (300, 1 << 20), (4096, 1 << 20)]
+HINTS = [(1, 1), (1, 1 << 20), (500, 1), (300, 1 << 20), (4096, 1 << 20)]
 
 
 def hinted(ops, b, hint):
