@@ -31,7 +31,7 @@
 //     tile on its way and one wave per SIMD measured better than more of either (129 against 111 us
 //     with four tiles in LDS, 188 against 108 us for Q8 at two waves per SIMD, which spills).
 //   many rows: the matrix units and the softmax between them (VALU).  Three prompts of 1001 .. 8192
-//     rows, f16, 32 / 8 heads, head_dim 128: 1205 - 1230 us = 950 - 970 TFLOP/s; one of 8192 rows, 8 / 4
+//     rows, f16, 32 / 8 heads, head_dim 128: 1213 us = 965 TFLOP/s; one of 8192 rows, 8 / 4
 //     heads, head_dim 256: 300 us = 900 TFLOP/s (409 us before its LDS reads went four products
 //     ahead of their use); 40 prompts of 9 .. 777 rows, bf16, 14 / 2 heads, head_dim 64: 36 us, a third
 //     of it short blocks' starts and ends.  At head_dim 256 a block's O, Q and S take a whole SIMD's
